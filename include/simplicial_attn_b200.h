@@ -171,6 +171,69 @@ int sa_resolve_algo(const sa_params* p);
  * changes the order of the sums, nothing else.  No counterpart in the reference. */
 int sa_general_plan(const sa_params* p);
 
+/* ---- Operators around the 2-simplicial layers of a model: rotary positions and ordinary causal attention.
+ * No counterpart in the reference, which starts at the projected tensors. */
+
+/* Rotary positions.  For every row (b, n) and rotated pair i of every head, with theta = position(b, n) * frequencies[i]:
+ *     (x, y) -> magnitude * (x cos theta - y sin theta, y cos theta + x sin theta)
+ * The pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) with `interleaved`; elements from rotary_dim on are copied.  With
+ * `inverse` the rotation is by -theta, which is the gradient of the call without it.  One launch serves up to four tensors
+ * [B, N, heads[t], D] with the same rows.  Angles are formed and reduced in 64 bits.
+ * `positions` is NULL (row n is at position `offset` + n) or holds 32- or 64-bit integers with element strides
+ * (position_b, position_n); `offset` is added.  `frequencies` holds rotary_dim / 2 radians per position (device memory,
+ * contiguous).  An output may be its input (same pointer and strides) and must not overlap it otherwise. */
+typedef struct {
+    int32_t tensors;             /* 1 to 4 */
+    int32_t B, N, D;
+    int32_t heads[4];
+    int32_t rotary_dim;          /* even, 2 .. D */
+    int32_t interleaved, inverse;
+    int32_t dtype;               /* sa_dtype of the tensors */
+    int32_t position_bits;       /* 32 or 64 (ignored without positions) */
+    int32_t frequency_bits;      /* 32 (float) or 64 (double) */
+    int64_t position_b, position_n, offset;
+    float magnitude;
+    sa_strides in[4], out[4];
+} sa_rotary_params;
+
+int sa_rotary(const sa_rotary_params* p, const void* const* in, void* const* out, const void* positions,
+              const void* frequencies, void* stream);
+
+/* Causal attention over whole prompts, packed sequences, chunks of a prompt or single tokens:
+ *     logits_ij = scale * sum_d Q_id * K_jd     over keys j <= i + (keys - queries) of i's sequence
+ *     O_i = sum_j softmax_j(logits_i) V_j;      LSE_i = log sum_j exp(logits_ij)
+ * so the last query of a sequence sees all its keys.  A query that sees none has O = 0 and LSE = -inf and takes part in no
+ * gradient.  Q, O are [B, Nq, H, D], K, V are [B, Nk, Hkv, D], LSE is [B, H, Nq] fp32 contiguous; head h reads KV head
+ * h / (H / Hkv).
+ * sequences == 0: every batch element is a sequence.  Otherwise B == 1 and sequence s is rows [cu_q[s], cu_q[s + 1]) of Q
+ * and [cu_k[s], cu_k[s + 1]) of K and V (device memory, `sequences` + 1 ints each, not decreasing; values are clipped to the
+ * tensors).  max_q / max_k say how long sequences are at most; they choose kernels and launch shapes, results are right
+ * whatever they say (0: as long as the tensor).  Rows outside every sequence get O = 0, LSE = -inf and zero gradients. */
+typedef struct {
+    int32_t B, Nq, Nk, H, Hkv, D;
+    int32_t sequences, max_q, max_k;
+    int32_t dtype, algo;         /* sa_dtype, sa_algo */
+    float scale;
+    sa_strides q, k, v, o;                    /* forward tensors (o also describes O in backward) */
+    sa_strides d_o, dq, dk, dv;               /* backward tensors (ignored by sa_causal_forward) */
+} sa_causal_params;
+
+/* `status`: see sa_forward_status.  `workspace`: sa_causal_*_workspace_size() bytes, 256-byte aligned; NULL where that is 0. */
+int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, const void* v, void* o, float* lse,
+                      const int32_t* cu_q, const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status,
+                      void* stream);
+/* dq, dk and dv may be NULL.  Gradients are overwritten, without atomics, in a fixed order. */
+int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, const void* v, const void* o,
+                       const float* lse, const void* d_o, void* dq, void* dk, void* dv, const int32_t* cu_q,
+                       const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status, void* stream);
+size_t sa_causal_forward_workspace_size(const sa_causal_params* p);
+size_t sa_causal_backward_workspace_size(const sa_causal_params* p);
+
+/* Which kernels AUTO takes for `p`, or a negative sa_status: SA_ALGO_GENERAL, SA_ALGO_TCGEN05, or for the forward
+ * SA_CAUSAL_FEW_ROWS (a few queries over many keys: single tokens).  Pointers are taken to be 16-byte aligned. */
+enum { SA_CAUSAL_FEW_ROWS = 3 };
+int sa_causal_resolve(const sa_causal_params* p, int backward);
+
 /* Strided copy between host and device (either direction, or device to device) on `stream`: `rows`
  * pieces of `row_bytes` bytes, `src_pitch` / `dst_pitch` bytes apart.  Used to move one group of
  * heads of a [B, N, H, D] tensor that lives in pinned host memory without staging it first.  Host

@@ -1,6 +1,8 @@
 """B200-native 2-simplicial attention: hand-written sm_100a CUDA kernels behind a C ABI, with the
 reference's operator interface on top (`TwoSimplicialAttention`,
-`TwoSimplicialAttentionFunction` and the kernel-named launchers).
+`TwoSimplicialAttentionFunction` and the kernel-named launchers), and the operators that a model needs around its
+2-simplicial layers: rotary positions (`rotary_positions`, `RotaryPositions`) and ordinary causal attention
+(`causal_attention`, `CausalSelfAttention`).
 
 The reference's package also re-exports its loop oracle and test runners
 (`simplicial/__init__.py:12-44`); those are test infrastructure and are not part of this library.
@@ -9,7 +11,9 @@ from .simplicial_attn import (TwoSimplicialAttention, TwoSimplicialAttentionFunc
                               two_simplicial_attention, two_simplicial_attn_bwd, two_simplicial_attn_bwd_kv1_kernel,
                               two_simplicial_attn_bwd_kv2_kernel, two_simplicial_attn_fwd_kernel)
 
-from .projection import TwoSimplicialSelfAttention
+from .causal_attn import CausalAttentionFunction, causal_attention, causal_attention_bwd, causal_attention_fwd
+from .projection import CausalSelfAttention, TwoSimplicialSelfAttention
+from .rotary import RotaryPositions, RotaryPositionsFunction, rotary_frequencies, rotary_positions
 
 _REFERENCE_ONLY = ("two_simplicial_attention_reference", "TwoSimplicialAttentionReference")
 
@@ -35,4 +39,13 @@ __all__ = [
     "compute_D_kernel",
     "check_device_status",
     "TwoSimplicialSelfAttention",
+    "CausalSelfAttention",
+    "causal_attention",
+    "causal_attention_fwd",
+    "causal_attention_bwd",
+    "CausalAttentionFunction",
+    "rotary_positions",
+    "rotary_frequencies",
+    "RotaryPositions",
+    "RotaryPositionsFunction",
 ]

@@ -15,11 +15,14 @@ SA_OK = 0
 SA_ERR_DEVICE_TIMEOUT = 7
 SA_BF16, SA_F16, SA_F32 = 0, 1, 2
 SA_ALGO_AUTO, SA_ALGO_GENERAL, SA_ALGO_TCGEN05 = 0, 1, 2
+SA_CAUSAL_FEW_ROWS = 3
 
 EXPORTS = ("sa_forward", "sa_backward", "sa_forward_workspace_size", "sa_backward_workspace_size", "sa_read_status",
            "sa_resolve_algo", "sa_strerror", "sa_version", "sa_kernel_launches", "sa_backward_static",
            "sa_backward_static_capacity", "sa_read_status_static", "sa_read_status_ex", "sa_set_wait_limit_ns",
-           "sa_selftest_wait_timeout", "sa_copy_rows_async", "sa_forward_status", "sa_backward_status", "sa_general_plan")
+           "sa_selftest_wait_timeout", "sa_copy_rows_async", "sa_forward_status", "sa_backward_status", "sa_general_plan",
+           "sa_rotary", "sa_causal_forward", "sa_causal_backward", "sa_causal_forward_workspace_size",
+           "sa_causal_backward_workspace_size", "sa_causal_resolve")
 
 
 class Strides(ctypes.Structure):
@@ -30,6 +33,18 @@ class Params(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_int32) for n in ("B", "N", "H", "Hkv", "D", "w1", "w2", "halo1", "halo2", "dtype", "algo")]
                 + [(n, ctypes.c_float) for n in ("scale", "k2_bias", "v2_bias")]
                 + [(n, Strides) for n in ("q", "k1", "k2", "v1", "v2", "o", "d_o", "dq", "dk1", "dk2", "dv1", "dv2")])
+
+
+class RotaryParams(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("tensors", "B", "N", "D")] + [("heads", ctypes.c_int32 * 4)]
+                + [(n, ctypes.c_int32) for n in ("rotary_dim", "interleaved", "inverse", "dtype", "position_bits", "frequency_bits")]
+                + [(n, ctypes.c_int64) for n in ("position_b", "position_n", "offset")] + [("magnitude", ctypes.c_float)]
+                + [("in", Strides * 4), ("out", Strides * 4)])
+
+
+class CausalParams(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("B", "Nq", "Nk", "H", "Hkv", "D", "sequences", "max_q", "max_k", "dtype", "algo")]
+                + [("scale", ctypes.c_float)] + [(n, Strides) for n in ("q", "k", "v", "o", "d_o", "dq", "dk", "dv")])
 
 
 class SimplicialAttnError(RuntimeError):
@@ -83,6 +98,19 @@ def load():
     lib.sa_selftest_wait_timeout.restype = ctypes.c_int
     lib.sa_copy_rows_async.argtypes = [vp, sz, vp, sz, sz, sz, vp]
     lib.sa_copy_rows_async.restype = ctypes.c_int
+    rp, cp = ctypes.POINTER(RotaryParams), ctypes.POINTER(CausalParams)
+    lib.sa_rotary.argtypes = [rp] + [vp] * 5
+    lib.sa_rotary.restype = ctypes.c_int
+    lib.sa_causal_forward.argtypes = [cp] + [vp] * 8 + [sz, vp, vp]
+    lib.sa_causal_forward.restype = ctypes.c_int
+    lib.sa_causal_backward.argtypes = [cp] + [vp] * 12 + [sz, vp, vp]
+    lib.sa_causal_backward.restype = ctypes.c_int
+    lib.sa_causal_forward_workspace_size.argtypes = [cp]
+    lib.sa_causal_forward_workspace_size.restype = sz
+    lib.sa_causal_backward_workspace_size.argtypes = [cp]
+    lib.sa_causal_backward_workspace_size.restype = sz
+    lib.sa_causal_resolve.argtypes = [cp, ctypes.c_int]
+    lib.sa_causal_resolve.restype = ctypes.c_int
     lib.sa_resolve_algo.argtypes = [pp]
     lib.sa_resolve_algo.restype = ctypes.c_int
     lib.sa_general_plan.argtypes = [pp]

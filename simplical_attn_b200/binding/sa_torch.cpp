@@ -1,4 +1,4 @@
-// The operator on torch tensors: argument checks, output allocation, the C-ABI call and the autograd node,
+// The operators on torch tensors (the 2-simplicial one here, the ones around it in sa_ops.h): argument checks, output allocation, the C-ABI call and the autograd node,
 // in one native call per direction.
 //
 // A small problem's kernels take about ten microseconds, so what the host does around them decides its speed.
@@ -21,14 +21,19 @@
 #include <cuda_runtime_api.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
 #include <atomic>
+#include <limits>
 #include <mutex>
+#include <string>
+#include <vector>
 
 #include "../../include/simplicial_attn_b200.h"
 
@@ -42,11 +47,12 @@ struct Config {
     int algo;
 };
 
-// ---- status words: pinned host memory, 256 bytes per device and direction ({code, wait site, block, 0})
+// ---- status words: pinned host memory, 256 bytes per device and kind of call ({code, wait site, block, 0})
 constexpr int kMaxDevices = 64;
 constexpr int kSlotInts = 64;
-enum Direction { kForward = 0, kBackward = 1 };
-const char* const kLabel[2] = {"sa_forward", "sa_backward"};
+enum Direction { kForward = 0, kBackward = 1, kCausalForward = 2, kCausalBackward = 3 };
+constexpr int kDirections = 4;
+const char* const kLabel[kDirections] = {"sa_forward", "sa_backward", "sa_causal_forward", "sa_causal_backward"};
 
 std::atomic<volatile int*> g_slots{nullptr};
 std::atomic<uint64_t> g_devices{0};               // bit per device that has been called on
@@ -59,14 +65,14 @@ volatile int* slot(int device, Direction d) {
         base = g_slots.load(std::memory_order_acquire);
         if (base == nullptr) {
             void* p = nullptr;
-            const size_t bytes = sizeof(int) * kSlotInts * 2 * kMaxDevices;
+            const size_t bytes = sizeof(int) * kSlotInts * kDirections * kMaxDevices;
             C10_CUDA_CHECK(cudaHostAlloc(&p, bytes, cudaHostAllocPortable | cudaHostAllocMapped));
             memset(p, 0, bytes);
             base = static_cast<volatile int*>(p);
             g_slots.store(base, std::memory_order_release);
         }
     }
-    return base + (device * 2 + d) * kSlotInts;
+    return base + (device * kDirections + d) * kSlotInts;
 }
 
 void* status_word(int device, Direction d) { return const_cast<int*>(slot(device, d)); }
@@ -87,7 +93,7 @@ PyObject* g_on_error = nullptr;       // Python callable (function name, status,
 // still runs, another of its blocks may give up and leave a second report.)
 void poll_device(int device) {
     g_devices.fetch_or(1ull << device, std::memory_order_relaxed);
-    for (Direction d : {kForward, kBackward}) {
+    for (Direction d : {kForward, kBackward, kCausalForward, kCausalBackward}) {
         volatile int* s = slot(device, d);
         if (s[0] != 0) {
             const int code = s[0], where = s[1], block = s[2];      // (the device writes the code last)
@@ -283,19 +289,19 @@ Config config_args(PyObject* const* a) {
     c.algo = (int)int_arg(a[7]);
     return c;
 }
-// Whether every one of the five inputs is a torch.Tensor or Parameter itself: what a subclass does with the tensors that
+// Whether every one of the first n inputs is a torch.Tensor or Parameter itself: what a subclass does with the tensors that
 // are allocated for it is up to its __torch_function__.
-bool exact(PyObject* const* a) {
-    for (int i = 0; i < 5; ++i)
+bool exact(PyObject* const* a, int n = 5) {
+    for (int i = 0; i < n; ++i)
         if (!THPVariable_CheckTypeExact(Py_TYPE(a[i]))) return false;
     return true;
 }
 // ... and the call is neither traced nor under a functorch transform, and no input carries a forward-mode tangent.
-bool plain(PyObject* const* a) {
-    if (!exact(a) || at::tracer::impl::is_dispatch_enabled() ||
+bool plain(PyObject* const* a, int n = 5) {
+    if (!exact(a, n) || at::tracer::impl::is_dispatch_enabled() ||
         c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode))
         return false;
-    for (int i = 0; i < 5; ++i) {
+    for (int i = 0; i < n; ++i) {
         const Tensor& t = THPVariable_Unpack(a[i]);
         if (t.unsafeGetTensorImpl()->autograd_meta() != nullptr && t._fw_grad(0).defined()) return false;
     }
@@ -381,12 +387,12 @@ PyObject* py_poll(PyObject*, PyObject* device) {
     END_HANDLE_TH_ERRORS
 }
 
-// device, direction (0: forward, 1: backward)
+// device, direction (0: forward, 1: backward, 2 and 3: the same of causal attention)
 PyObject* py_status_word(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     expect(n, 2);
     const int64_t device = int_arg(a[0]), direction = int_arg(a[1]);
-    TORCH_CHECK_INDEX(device >= 0 && device < kMaxDevices && (direction == kForward || direction == kBackward), "no such status word");
+    TORCH_CHECK_INDEX(device >= 0 && device < kMaxDevices && direction >= 0 && direction < kDirections, "no such status word");
     return PyLong_FromVoidPtr(status_word((int)device, (Direction)direction));
     END_HANDLE_TH_ERRORS
 }
@@ -409,11 +415,17 @@ PyObject* py_on_error(PyObject*, PyObject* fn) {
     Py_RETURN_NONE;
 }
 
+#include "sa_ops.h"
+
 PyMethodDef kMethods[] = {
     {"attention", (PyCFunction)(void*)py_attention, METH_FASTCALL, "O with its autograd history; None if the call is not plain"},
     {"plain", (PyCFunction)(void*)py_plain, METH_FASTCALL, "whether `attention` makes the call for these five inputs"},
     {"forward", (PyCFunction)(void*)py_forward, METH_FASTCALL, "(O, LSE); None for tensor subclasses"},
     {"backward", (PyCFunction)(void*)py_backward, METH_FASTCALL, "(dq, dk1, dk2, dv1, dv2); None for tensor subclasses"},
+    {"rotary", (PyCFunction)(void*)py_rotary, METH_FASTCALL, "the rotated tensors with their autograd history; None if the call is not plain"},
+    {"causal_attention", (PyCFunction)(void*)py_causal, METH_FASTCALL, "(O, LSE), O with its autograd history; None if the call is not plain"},
+    {"causal_forward", (PyCFunction)(void*)py_causal_forward, METH_FASTCALL, "(O, LSE); None for tensor subclasses"},
+    {"causal_backward", (PyCFunction)(void*)py_causal_backward, METH_FASTCALL, "(dq, dk, dv); None for tensor subclasses"},
     {"poll", py_poll, METH_O, "raises if an earlier call on the device left a status"},
     {"status_word", (PyCFunction)(void*)py_status_word, METH_FASTCALL, "address of the word that calls of a device and direction report to"},
     {"devices", py_devices, METH_NOARGS, "indices of the devices that have been called on"},

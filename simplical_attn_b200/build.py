@@ -100,6 +100,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 # ---- the torch binding: host code only, compiled by the C++ compiler against torch's headers
 BINDING_SRC = os.path.join(PKG, "binding", "sa_torch.cpp")
+BINDING_HEADER = os.path.join(PKG, "binding", "sa_ops.h")       # included by it
 BINDING = os.path.join(LIB_DIR, "sa_torch.so")
 BINDING_STAMP = BINDING + ".sources"
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
@@ -118,7 +119,7 @@ def have_host_compiler() -> bool:
 def binding_digest() -> str:
     import torch
     h = hashlib.sha256(" ".join(CXX_FLAGS + [torch.__version__, sys.version]).encode())
-    for d in (BINDING_SRC, os.path.join(os.path.dirname(PKG), "include", "simplicial_attn_b200.h")):
+    for d in (BINDING_SRC, BINDING_HEADER, os.path.join(os.path.dirname(PKG), "include", "simplicial_attn_b200.h")):
         with open(d, "rb") as f:
             h.update(f.read())
     return h.hexdigest()

@@ -9,6 +9,7 @@
 
 #include "sa_common.cuh"
 #include "sa_general.cuh"
+#include "sa_host.cuh"
 #include "sa_tc_bwd.cuh"
 #include "sa_tc_fwd.cuh"
 
@@ -420,9 +421,23 @@ int resolve(const sa_params* p, bool backward) {
 
 }  // namespace
 
+namespace sa {
+namespace host {
+
+void count_launches(int n) { g_launches += n; }
+uint64_t wait_limit_ns() { return g_wait_limit_ns.load(); }
+int sm_count() { return plan_sm_count(); }
+int cc_major() { return device_info().cc_major; }
+bool make_map(CUtensorMap* map, const void* base, int B, int rows, int heads, int D, const sa_strides& st, int box_rows, bool f16) {
+    return ::make_map(map, base, B, rows, heads, D, st, box_rows, f16);
+}
+
+}  // namespace host
+}  // namespace sa
+
 extern "C" {
 
-int sa_version(void) { return 300; }
+int sa_version(void) { return 400; }
 
 uint64_t sa_kernel_launches(void) { return g_launches.load(); }
 

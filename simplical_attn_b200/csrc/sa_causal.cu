@@ -1,0 +1,115 @@
+// C entries of causal attention: argument validation, kernel selection and launches.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "sa_causal.cuh"
+#include "sa_causal_general.cuh"
+
+namespace sa {
+namespace causal {
+namespace {
+
+int validate(const sa_causal_params* p) {
+    if (!p) return SA_ERR_NULL_POINTER;
+    if (p->B < 1 || p->Nq < 1 || p->Nk < 1 || p->H < 1 || p->Hkv < 1 || p->D < 1 || p->H % p->Hkv != 0) return SA_ERR_BAD_SHAPE;
+    if (p->sequences < 0 || p->max_q < 0 || p->max_k < 0 || (p->sequences > 0 && p->B != 1)) return SA_ERR_BAD_SHAPE;
+    if (p->dtype < SA_BF16 || p->dtype > SA_F32 || p->D > 256) return SA_ERR_UNSUPPORTED;
+    if (p->algo < SA_ALGO_AUTO || p->algo > SA_ALGO_TCGEN05) return SA_ERR_UNSUPPORTED;
+    if (p->Nq > (1 << 30) || p->Nk > (1 << 30) || (int64_t)p->H * (p->sequences > 0 ? p->sequences : p->B) > (1 << 30)) return SA_ERR_UNSUPPORTED;
+    return SA_OK;
+}
+
+CParams make_params(const sa_causal_params* p, const int32_t* cu_q, const int32_t* cu_k) {
+    CParams c{};
+    c.B = p->B; c.Nq = p->Nq; c.Nk = p->Nk; c.H = p->H; c.Hkv = p->Hkv; c.D = p->D; c.G = p->H / p->Hkv;
+    c.S = p->sequences > 0 ? p->sequences : p->B;
+    c.max_q = p->sequences > 0 && p->max_q > 0 && p->max_q < p->Nq ? p->max_q : p->Nq;
+    c.max_k = p->sequences > 0 && p->max_k > 0 && p->max_k < p->Nk ? p->max_k : p->Nk;
+    c.cu_q = cu_q; c.cu_k = cu_k;
+    c.scale = p->scale;
+    c.q = p->q; c.k = p->k; c.v = p->v; c.o = p->o; c.d_o = p->d_o; c.dq = p->dq; c.dk = p->dk; c.dv = p->dv;
+    // the stride of an extent of one is never used
+    auto fix = [](sa_strides& s, int b, int n, int h) {
+        if (b == 1) s.b = 0;
+        if (n == 1) s.n = 0;
+        if (h == 1) s.h = 0;
+    };
+    for (sa_strides* s : {&c.q, &c.o, &c.d_o, &c.dq}) fix(*s, c.B, c.Nq, c.H);
+    for (sa_strides* s : {&c.k, &c.v, &c.dk, &c.dv}) fix(*s, c.B, c.Nk, c.Hkv);
+    return c;
+}
+
+int resolve(const sa_causal_params* p, bool backward) {
+    (void)backward;
+    if (p->algo == SA_ALGO_TCGEN05) return -SA_ERR_UNSUPPORTED;
+    return SA_ALGO_GENERAL;
+}
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+size_t delta_bytes(const sa_causal_params* p) { return align256((size_t)p->B * p->H * p->Nq * sizeof(float)); }
+
+bool workspace_ok(const void* ws, size_t bytes, size_t need) {
+    if (need == 0) return true;
+    return ws != nullptr && bytes >= need && (reinterpret_cast<uintptr_t>(ws) & 255u) == 0;
+}
+
+}  // namespace
+}  // namespace causal
+}  // namespace sa
+
+extern "C" {
+
+size_t sa_causal_forward_workspace_size(const sa_causal_params* p) {
+    using namespace sa::causal;
+    if (validate(p) != SA_OK) return 0;
+    return 0;
+}
+
+size_t sa_causal_backward_workspace_size(const sa_causal_params* p) {
+    using namespace sa::causal;
+    if (validate(p) != SA_OK) return 0;
+    return delta_bytes(p);
+}
+
+int sa_causal_resolve(const sa_causal_params* p, int backward) {
+    using namespace sa::causal;
+    const int rc = validate(p);
+    return rc != SA_OK ? -rc : resolve(p, backward != 0);
+}
+
+int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* cu_q,
+                      const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status, void* stream) {
+    using namespace sa::causal;
+    int rc = validate(p);
+    if (rc != SA_OK) return rc;
+    if (!q || !k || !v || !o || !lse || !status || (p->sequences > 0 && (!cu_q || !cu_k))) return SA_ERR_NULL_POINTER;
+    if (!workspace_ok(workspace, workspace_bytes, sa_causal_forward_workspace_size(p)) || !sa::host::aligned16(status)) return SA_ERR_WORKSPACE;
+    const int algo = resolve(p, false);
+    if (algo < 0) return -algo;
+    const CParams c = make_params(p, p->sequences > 0 ? cu_q : nullptr, p->sequences > 0 ? cu_k : nullptr);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dispatch_general(p->dtype, p->D, [&](auto t, auto d) { return launch_general_fwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, lse, st); });
+}
+
+int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o,
+                       void* dq, void* dk, void* dv, const int32_t* cu_q, const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status,
+                       void* stream) {
+    using namespace sa::causal;
+    int rc = validate(p);
+    if (rc != SA_OK) return rc;
+    if (!q || !k || !v || !o || !lse || !d_o || !status || (p->sequences > 0 && (!cu_q || !cu_k))) return SA_ERR_NULL_POINTER;
+    if (!workspace_ok(workspace, workspace_bytes, sa_causal_backward_workspace_size(p)) || !sa::host::aligned16(status)) return SA_ERR_WORKSPACE;
+    if (!dq && !dk && !dv) return SA_OK;
+    const int algo = resolve(p, true);
+    if (algo < 0) return -algo;
+    const CParams c = make_params(p, p->sequences > 0 ? cu_q : nullptr, p->sequences > 0 ? cu_k : nullptr);
+    float* delta = static_cast<float*>(workspace);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dispatch_general(p->dtype, p->D, [&](auto t, auto d) {
+        return launch_general_bwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, lse, d_o, dq, dk, dv, delta, st);
+    });
+}
+
+}  // extern "C"

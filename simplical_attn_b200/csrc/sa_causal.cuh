@@ -1,0 +1,71 @@
+// Definitions shared by the causal attention kernels: the problem, its sequences, rows outside of them.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "sa_common.cuh"
+#include "sa_host.cuh"
+
+namespace sa {
+namespace causal {
+
+// Problem descriptor handed to every kernel by value.
+struct CParams {
+    int B, Nq, Nk, H, Hkv, D, G;         // G = H / Hkv query heads per KV head
+    int S;                               // sequences; without cu_q those are the batch elements
+    int max_q, max_k;                    // bounds of the lengths, for launch shapes only
+    const int* cu_q;                     // NULL: every batch element is a sequence
+    const int* cu_k;
+    float scale;
+    sa_strides q, k, v, o, d_o, dq, dk, dv;
+};
+
+// Rows of one sequence: queries [q0, q0 + nq) and keys [k0, k0 + nk) of batch element b.  Query i (from 0) sees keys
+// j <= i + off, off = nk - nq.
+struct Seq {
+    int b, q0, nq, k0, nk;
+    __device__ __forceinline__ int off() const { return nk - nq; }
+};
+
+// Whatever cu_q and cu_k hold, the rows are rows of the tensors.
+__device__ __forceinline__ void clipped(const int* cu, int s, int n, int& start, int& len) {
+    start = min(max(cu[s], 0), n);
+    len = min(max(cu[s + 1], start), n) - start;
+}
+__device__ __forceinline__ Seq seq_of(const CParams& p, int s) {
+    Seq r;
+    if (p.cu_q == nullptr) {
+        r.b = s;
+        r.q0 = r.k0 = 0;
+        r.nq = p.Nq;
+        r.nk = p.Nk;
+    } else {
+        r.b = 0;
+        clipped(p.cu_q, s, p.Nq, r.q0, r.nq);
+        clipped(p.cu_k, s, p.Nk, r.k0, r.nk);
+    }
+    return r;
+}
+
+// Zeroes the rows of a packed tensor before the first and behind the last sequence (there are none as a rule: two loads).
+// `block` of `blocks` equal shares, every thread of the block takes part.
+template <typename T>
+__device__ __forceinline__ void zero_outside(T* x, const sa_strides& st, int heads, int D, int n, const int* cu, int S, int block, int blocks) {
+    const int first = min(max(cu[0], 0), n), last = max(min(max(cu[S], 0), n), first);
+    const int out = first + n - last;
+    for (int i = block; i < out; i += blocks) {
+        T* row = x + (int64_t)(i < first ? i : last + i - first) * st.n;
+        for (int e = threadIdx.x; e < heads * D; e += blockDim.x) row[(int64_t)(e / D) * st.h + e % D] = from_f<T>(0.f);
+    }
+}
+__device__ __forceinline__ void empty_lse_outside(float* lse, int H, int n, const int* cu, int S, int block, int blocks) {
+    const int first = min(max(cu[0], 0), n), last = max(min(max(cu[S], 0), n), first);
+    const int out = first + n - last;
+    for (int i = block; i < out; i += blocks)
+        for (int h = threadIdx.x; h < H; h += blockDim.x) lse[(int64_t)h * n + (i < first ? i : last + i - first)] = -INFINITY;
+}
+
+inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+}  // namespace causal
+}  // namespace sa

@@ -1,0 +1,243 @@
+// Rotary positions (sa_rotary): every pair (x, y) of the rotated part of a head turned by position * frequency.
+//
+// The kernel moves every element once and computes about three flops for it: HBM bandwidth bounds it, launch latency where
+// there are few rows.  Nothing is tabulated: an angle is formed from the position and the frequency, so any position works
+// and no table is read.  The product is taken and reduced to an eighth of a turn in 64 bits (in 32 a position of 10^6 would be
+// off by 0.06 radians), sine and cosine of the remainder in 32.  A thread keeps its sines and cosines for up to four heads,
+// whose loads are all in flight before the first is used.
+#include <cuda_runtime.h>
+
+#include "sa_common.cuh"
+#include "sa_host.cuh"
+
+namespace sa {
+namespace rotary {
+
+constexpr int kThreads = 256;
+constexpr int kHeads = 4;            // heads a thread turns by the same angles
+constexpr int kMaxTensors = 4;
+
+struct Params {
+    const void* in[kMaxTensors];
+    void* out[kMaxTensors];
+    sa_strides si[kMaxTensors], so[kMaxTensors];
+    int heads[kMaxTensors];
+    int blocks_end[kMaxTensors];     // head blocks of the tensors up to this one
+    int tensors, N, D, rd;
+    unsigned rows, head_blocks, groups, turned_groups;       // groups: of 2 V elements of a head
+    const void* positions;
+    const void* frequencies;
+    int position_bits, frequency_bits;
+    int64_t position_b, position_n, offset;
+    float magnitude;
+    int inverse;
+};
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+    T e[V];
+};
+
+// cos and sin of a whole turn's fraction given in quarter turns: the nearest whole number of quarters is taken off in 64
+// bits, so that the 32-bit remainder is at most an eighth of a turn and its rounding at most 2^-25 quarters.
+__device__ __forceinline__ void cos_sin_quarters(double quarters, float& c, float& s) {
+    const double n = rint(quarters);
+    float sr, cr;
+    sincospif(0.5f * (float)(quarters - n), &sr, &cr);
+    const int k = (int)(n - 4.0 * floor(0.25 * n));        // n modulo 4
+    c = (k & 1) ? sr : cr;
+    s = (k & 1) ? cr : sr;
+    if (k == 1 || k == 2) c = -c;
+    if (k >= 2) s = -s;
+}
+
+template <typename T, int V, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ Params p) {
+    unsigned idx = blockIdx.x * kThreads + threadIdx.x;
+    const unsigned g = idx % p.groups;
+    idx /= p.groups;
+    const unsigned hb = idx % p.head_blocks, row = idx / p.head_blocks;
+    if (row >= p.rows) return;
+    const unsigned b = row / (unsigned)p.N, n = row - b * (unsigned)p.N;
+
+    int t = 0, first_block = 0;
+#pragma unroll
+    for (int x = 0; x < kMaxTensors - 1; ++x)
+        if (x + 1 < p.tensors && (int)hb >= p.blocks_end[x]) {
+            t = x + 1;
+            first_block = p.blocks_end[x];
+        }
+    // (selected by comparisons: an index that is not a constant would copy the parameters to local memory)
+    const void* in = p.in[0];
+    void* out = p.out[0];
+    sa_strides si = p.si[0], so = p.so[0];
+    int heads = p.heads[0];
+#pragma unroll
+    for (int x = 1; x < kMaxTensors; ++x)
+        if (t == x) {
+            in = p.in[x];
+            out = p.out[x];
+            si = p.si[x];
+            so = p.so[x];
+            heads = p.heads[x];
+        }
+    const int h0 = ((int)hb - first_block) * kHeads, nh = min(kHeads, heads - h0);
+
+    // the two vectors of this group within a head
+    const bool turned = g < p.turned_groups;
+    int oa, ob;
+    if (!turned) {
+        oa = p.rd + (int)(g - p.turned_groups) * 2 * V;
+        ob = oa + V;
+    } else if (INTERLEAVED) {
+        oa = (int)g * 2 * V;
+        ob = oa + V;
+    } else {
+        oa = (int)g * V;
+        ob = p.rd / 2 + oa;
+    }
+    const bool have_b = ob < p.D;
+    const T* src = (const T*)in + (int64_t)b * si.b + (int64_t)n * si.n + (int64_t)h0 * si.h;
+    T* dst = (T*)out + (int64_t)b * so.b + (int64_t)n * so.n + (int64_t)h0 * so.h;
+    if (!turned && src == dst) return;
+
+    using W = Vec<T, V>;
+    W a[kHeads], c[kHeads];
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
+        if (h < nh) {
+            a[h] = *reinterpret_cast<const W*>(src + h * si.h + oa);
+            if (have_b) c[h] = *reinterpret_cast<const W*>(src + h * si.h + ob);
+        }
+    if (turned) {
+        int64_t at = p.offset;
+        if (p.positions == nullptr) at += n;
+        else {
+            const int64_t i = (int64_t)b * p.position_b + (int64_t)n * p.position_n;
+            at += p.position_bits == 64 ? ((const int64_t*)p.positions)[i] : (int64_t)((const int32_t*)p.positions)[i];
+        }
+        const double quarters = (double)at * 0.63661977236758134308;         // 2 / pi
+        float cs[V], sn[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const int i = (int)g * V + e;
+            const double f = p.frequency_bits == 64 ? ((const double*)p.frequencies)[i] : (double)((const float*)p.frequencies)[i];
+            cos_sin_quarters(quarters * f, cs[e], sn[e]);
+            cs[e] *= p.magnitude;
+            sn[e] *= p.inverse ? -p.magnitude : p.magnitude;
+        }
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h)
+            if (h < nh) {
+                T x[2 * V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    x[e] = a[h].e[e];
+                    x[V + e] = c[h].e[e];
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const int ix = INTERLEAVED ? 2 * e : e, iy = INTERLEAVED ? 2 * e + 1 : V + e;
+                    const float u = to_f<T>(x[ix]), w = to_f<T>(x[iy]);
+                    x[ix] = from_f<T>(u * cs[e] - w * sn[e]);
+                    x[iy] = from_f<T>(w * cs[e] + u * sn[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    a[h].e[e] = x[e];
+                    c[h].e[e] = x[V + e];
+                }
+            }
+    }
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
+        if (h < nh) {
+            *reinterpret_cast<W*>(dst + h * so.h + oa) = a[h];
+            if (have_b) *reinterpret_cast<W*>(dst + h * so.h + ob) = c[h];
+        }
+}
+
+template <typename T, int V>
+int launch_v(Params& p, bool interleaved, cudaStream_t st) {
+    p.turned_groups = (unsigned)(p.rd / (2 * V));
+    p.groups = p.turned_groups + (unsigned)((p.D - p.rd + 2 * V - 1) / (2 * V));
+    const uint64_t threads = (uint64_t)p.rows * p.head_blocks * p.groups;
+    if (threads > 0x7fffffffull - kThreads) return SA_ERR_UNSUPPORTED;
+    const unsigned grid = (unsigned)((threads + kThreads - 1) / kThreads);
+    if (interleaved) rotary_kernel<T, V, true><<<grid, kThreads, 0, st>>>(p);
+    else rotary_kernel<T, V, false><<<grid, kThreads, 0, st>>>(p);
+    host::count_launches(1);
+    return cudaGetLastError() == cudaSuccess ? SA_OK : SA_ERR_LAUNCH;
+}
+
+// The widest vectors (up to 16 bytes) that every address of the call allows.
+template <typename T>
+int launch_t(Params& p, bool interleaved, cudaStream_t st) {
+    auto fits = [&](int v) {
+        if (p.rd % (2 * v) != 0 || p.D % v != 0) return false;
+        for (int t = 0; t < p.tensors; ++t) {
+            if (reinterpret_cast<uintptr_t>(p.in[t]) % (v * sizeof(T)) != 0 || reinterpret_cast<uintptr_t>(p.out[t]) % (v * sizeof(T)) != 0) return false;
+            for (const sa_strides* s : {&p.si[t], &p.so[t]})
+                if (s->b % v != 0 || s->n % v != 0 || s->h % v != 0) return false;
+        }
+        return true;
+    };
+    if constexpr (sizeof(T) == 2)
+        if (fits(8)) return launch_v<T, 8>(p, interleaved, st);
+    if (fits(4)) return launch_v<T, 4>(p, interleaved, st);
+    if (fits(2)) return launch_v<T, 2>(p, interleaved, st);
+    return launch_v<T, 1>(p, interleaved, st);
+}
+
+}  // namespace rotary
+}  // namespace sa
+
+extern "C" int sa_rotary(const sa_rotary_params* p, const void* const* in, void* const* out, const void* positions,
+                         const void* frequencies, void* stream) {
+    using namespace sa::rotary;
+    if (!p || !in || !out || !frequencies) return SA_ERR_NULL_POINTER;
+    if (p->tensors < 1 || p->tensors > kMaxTensors || p->B < 1 || p->N < 1 || p->D < 1) return SA_ERR_BAD_SHAPE;
+    if (p->rotary_dim < 2 || p->rotary_dim > p->D || p->rotary_dim % 2 != 0) return SA_ERR_BAD_SHAPE;
+    if (p->dtype < SA_BF16 || p->dtype > SA_F32) return SA_ERR_UNSUPPORTED;
+    if (p->frequency_bits != 32 && p->frequency_bits != 64) return SA_ERR_UNSUPPORTED;
+    if (positions && p->position_bits != 32 && p->position_bits != 64) return SA_ERR_UNSUPPORTED;
+    if ((int64_t)p->B * p->N > 0x7fffffffll) return SA_ERR_UNSUPPORTED;
+    Params k{};
+    int blocks = 0;
+    for (int t = 0; t < p->tensors; ++t) {
+        if (!in[t] || !out[t]) return SA_ERR_NULL_POINTER;
+        if (p->heads[t] < 1) return SA_ERR_BAD_SHAPE;
+        k.in[t] = in[t];
+        k.out[t] = out[t];
+        k.si[t] = p->in[t];
+        k.so[t] = p->out[t];
+        for (sa_strides* x : {&k.si[t], &k.so[t]}) {       // the stride of an extent of one is never used
+            if (p->B == 1) x->b = 0;
+            if (p->N == 1) x->n = 0;
+            if (p->heads[t] == 1) x->h = 0;
+        }
+        k.heads[t] = p->heads[t];
+        blocks += (p->heads[t] + kHeads - 1) / kHeads;
+        k.blocks_end[t] = blocks;
+    }
+    k.tensors = p->tensors;
+    k.N = p->N;
+    k.D = p->D;
+    k.rd = p->rotary_dim;
+    k.rows = (unsigned)(p->B * p->N);
+    k.head_blocks = (unsigned)blocks;
+    k.positions = positions;
+    k.frequencies = frequencies;
+    k.position_bits = p->position_bits;
+    k.frequency_bits = p->frequency_bits;
+    k.position_b = p->position_b;
+    k.position_n = p->position_n;
+    k.offset = p->offset;
+    k.magnitude = p->magnitude;
+    k.inverse = p->inverse != 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool il = p->interleaved != 0;
+    if (p->dtype == SA_BF16) return launch_t<__nv_bfloat16>(k, il, st);
+    if (p->dtype == SA_F16) return launch_t<__half>(k, il, st);
+    return launch_t<float>(k, il, st);
+}
