@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "sa_causal.cuh"
+#include "sa_causal_fwd.cuh"
 #include "sa_causal_general.cuh"
 
 namespace sa {
@@ -41,10 +42,38 @@ CParams make_params(const sa_causal_params* p, const int32_t* cu_q, const int32_
     return c;
 }
 
+// Whether the tensor-core kernels cover the problem (pointers and what a tensor map can hold are looked at in the call).
+bool tc_ok(const sa_causal_params* p, bool backward) {
+    if (backward) return false;
+    if (p->dtype == SA_F32 || (p->D != 64 && p->D != 128)) return false;
+    if (!(p->scale > 0.f)) return false;            // the row maximum is taken before scaling
+    const CParams c = make_params(p, nullptr, nullptr);
+    for (const sa_strides* s : {&c.q, &c.k, &c.v, &c.o})
+        if (!host::strides8(*s)) return false;
+    if (backward)
+        for (const sa_strides* s : {&c.d_o, &c.dq, &c.dk, &c.dv})
+            if (!host::strides8(*s)) return false;
+    return true;
+}
+
 int resolve(const sa_causal_params* p, bool backward) {
-    (void)backward;
-    if (p->algo == SA_ALGO_TCGEN05) return -SA_ERR_UNSUPPORTED;
-    return SA_ALGO_GENERAL;
+    const bool ok = p->algo != SA_ALGO_GENERAL && tc_ok(p, backward);
+    if (p->algo == SA_ALGO_TCGEN05 && !ok) return -SA_ERR_UNSUPPORTED;
+    return ok ? SA_ALGO_TCGEN05 : SA_ALGO_GENERAL;
+}
+
+// (a plan only asks whether there are starts)
+const int32_t* const kSomeStarts = reinterpret_cast<const int32_t*>(64);
+CParams planned(const sa_causal_params* p) {
+    const int32_t* cu = p->sequences > 0 ? kSomeStarts : nullptr;
+    return make_params(p, cu, cu);
+}
+
+// f(head dim, element type) of the tensor-core kernels
+template <typename F>
+int dispatch_tc(const sa_causal_params* p, F&& f) {
+    auto by_type = [&](auto d) { return p->dtype == SA_F16 ? f(d, std::true_type{}) : f(d, std::false_type{}); };
+    return p->D == 128 ? by_type(std::integral_constant<int, 128>{}) : by_type(std::integral_constant<int, 64>{});
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -63,8 +92,8 @@ extern "C" {
 
 size_t sa_causal_forward_workspace_size(const sa_causal_params* p) {
     using namespace sa::causal;
-    if (validate(p) != SA_OK) return 0;
-    return 0;
+    if (validate(p) != SA_OK || resolve(p, false) != SA_ALGO_TCGEN05) return 0;
+    return plan_fwd(planned(p)).bytes;
 }
 
 size_t sa_causal_backward_workspace_size(const sa_causal_params* p) {
@@ -90,6 +119,17 @@ int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, c
     if (algo < 0) return -algo;
     const CParams c = make_params(p, p->sequences > 0 ? cu_q : nullptr, p->sequences > 0 ? cu_k : nullptr);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (algo == SA_ALGO_TCGEN05) {
+        if (sa::host::cc_major() != 10) return SA_ERR_NOT_SM100;
+        rc = SA_ERR_BAD_STRIDE;
+        if (sa::host::aligned16(q) && sa::host::aligned16(k) && sa::host::aligned16(v) && sa::host::aligned16(o))
+            rc = dispatch_tc(p, [&](auto d, auto f16) {
+                return launch_fwd_tc<decltype(d)::value, decltype(f16)::value>(c, q, k, v, o, lse, static_cast<uint8_t*>(workspace),
+                                                                             static_cast<sa::DeviceStatus*>(status), st);
+            });
+        // (BAD_STRIDE: nothing has been launched)
+        if (rc != SA_ERR_BAD_STRIDE || p->algo == SA_ALGO_TCGEN05) return rc;
+    }
     return dispatch_general(p->dtype, p->D, [&](auto t, auto d) { return launch_general_fwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, lse, st); });
 }
 

@@ -65,7 +65,7 @@ __device__ __forceinline__ void empty_lse_outside(float* lse, int H, int n, cons
         for (int h = threadIdx.x; h < H; h += blockDim.x) lse[(int64_t)h * n + (i < first ? i : last + i - first)] = -INFINITY;
 }
 
-inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+__host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 }  // namespace causal
 }  // namespace sa

@@ -1,0 +1,663 @@
+// Causal attention forward on the sm_100a tensor cores (bf16 / fp16, head dim 64 and 128).
+//
+//     S = Q K^T,  P = exp2(S scale log2e - m),  O = sum over key tiles of P V / l,  with the running maximum m and sum l per row.
+//
+// A unit is a pair of 128-query tiles of one head (and one share of the keys); persistent blocks, one per multiprocessor, take
+// the units from the most to the least expensive in alternating direction.  Both query tiles stream through the same
+// 128-key tiles of K and V.
+//
+// Warps.  0-3 / 4-7: softmax group of query tile 0 / 1, a row per thread, also writes the rows out.  8: MMA issuer.  9: TMA.
+// 10: V guard (see below).  The query tiles work in opposite phase: while one is in its softmax the tensor cores work for the
+// other.  The issuer's loop runs on over units: S of the next unit's first tile is computed while the rows are written out.
+// Tensor memory: S0 | S1 (128 columns each; P overwrites S as packed 16-bit values) | O0 | O1 (D columns).
+//
+// Per pair of query tiles and 128 keys at D = 128 the MMAs take 2048 cycles (128 x 128 x 16 in 64) and so do the exponentials
+// (16 per clock): see the measured figures at the launch.
+//
+// Masked scores become -inf whatever they are, so P is an exact zero there; V rows of tiles with masked scores might still meet
+// that zero as NaN or infinity.  The guard warp looks through those tiles before their MMAs: rows behind the sequence's
+// keys become zeros, and an element that is not finite becomes a zero whose row is noted per column; the epilogue puts the
+// infinity or NaN back into the rows that see it.
+#pragma once
+
+#include "sa_causal_tc.cuh"
+
+namespace sa {
+namespace causal {
+
+constexpr int kFwdThreads = 384;
+constexpr int kFwdRegsSoftmax = 208, kFwdRegsRest = 88;
+static_assert(2 * kFwdRegsSoftmax + kFwdRegsRest <= 3 * 168, "register pool of the block (384 x 168 at launch)");
+constexpr float kRescaleLog2 = 8.0f;      // the running maximum is kept until a score exceeds it by this much (log2)
+
+struct FwdParams {
+    CParams c;
+    WorkList work;            // tiles of 128 row_tiles queries
+    int row_tiles;            // query tiles of a unit: 2, or 1 where that spreads a small problem over more multiprocessors
+    int splits;               // shares of the keys of a pair
+    float* part_o;            // splits > 1: [splits][B H Nq][D] partial rows, and their LSE [splits][B H Nq]
+    float* part_lse;
+    DeviceStatus* status;
+    uint64_t wait_limit_ns;
+};
+
+template <int HD>
+struct FwdLayout {
+    static constexpr int kSlabs = HD / 64;
+    static constexpr int kSlab = kTile * 128;                    // bytes of a [128 x 64] slab
+    static constexpr int kTileBytes = kSlabs * kSlab;
+    static constexpr int kStages = HD == 128 ? 5 : 8;            // ring of K and V tiles
+    static constexpr int kMisc = 320;                            // behind the barriers
+    static constexpr int kBad = 512;                             // guard: [3][HD] first rows that hold +inf, -inf, NaN
+    static constexpr int kQ = 2048;
+    static constexpr int kRing = kQ + 2 * kTileBytes;
+    static constexpr int kBytes = kRing + kStages * kTileBytes + 1024;       // 1024: alignment of the base
+    static_assert(kBad + 3 * HD * 4 <= kQ && kQ % 1024 == 0 && kBytes <= 227 * 1024, "shared memory of a block");
+};
+
+// A unit: query tiles r = 0, 1 at rows i0 + 128 r take key tiles [t0, t0 + m[r]).
+struct FwdUnit {
+    Seq s;
+    int h, split, i0, t0, m0, m1;
+    __device__ __forceinline__ int m(int r) const { return r ? m1 : m0; }
+    __device__ __forceinline__ int tiles() const { return max(m0, m1); }
+    // first key tile (counted from t0) in which row i0 + 128 r does not see every key
+    __device__ __forceinline__ int first_masked(int r) const {
+        const int limit = i0 + kTile * r + s.off() + 1;           // keys that row sees
+        return max((limit > 0 ? limit : 0) / kTile - t0, 0);
+    }
+};
+
+struct FwdWalk {
+    int u, round, count;
+    __device__ __forceinline__ explicit FwdWalk(const FwdParams& P) {
+        count = list_count(P.work) * P.c.H * P.splits;
+        round = 0;
+        u = blockIdx.x;
+    }
+    __device__ __forceinline__ bool valid() const { return u < count; }
+    __device__ __forceinline__ void next() {
+        ++round;
+        u = round * (int)gridDim.x + ((round & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+    }
+    __device__ __forceinline__ FwdUnit unit(const FwdParams& P) const {
+        FwdUnit r;
+        const int x = u / P.splits, item = x / P.c.H;
+        r.split = u - x * P.splits;
+        r.h = x - item * P.c.H;
+        int tile;
+        list_item(P.c, P.work, item, r.s, tile);
+        r.i0 = tile * P.row_tiles * kTile;
+        const int n0 = key_tiles(r.i0, kTile, r.s.nq, r.s.nk), n1 = P.row_tiles > 1 ? key_tiles(r.i0 + kTile, kTile, r.s.nq, r.s.nk) : 0;
+        const int share = (max(n0, n1) + P.splits - 1) / P.splits;
+        r.t0 = r.split * share;
+        r.m0 = min(max(n0 - r.t0, 0), share);
+        r.m1 = min(max(n1 - r.t0, 0), share);
+        return r;
+    }
+};
+
+struct Ring {
+    int s = 0;
+    uint32_t phase = 0;
+    template <int N>
+    __device__ __forceinline__ void next() {
+        if (++s == N) {
+            s = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+template <int HD, bool F16>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                     const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ o, float* __restrict__ lse) {
+    using L = FwdLayout<HD>;
+    using namespace ptx;
+    using E = El<F16>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t base = smem_u32(smem);
+    const CParams& p = P.c;
+
+    constexpr int kFull = 0;                          // [stage] K or V tile landed
+    constexpr int kEmpty = kFull + 8 * L::kStages;    //         read by the MMAs and passed by the guard
+    constexpr int kPassed = kEmpty + 8 * L::kStages;  //         looked through by the guard
+    constexpr int kQFull = kPassed + 8 * L::kStages;  // [query tile] Q landed
+    constexpr int kQFree = kQFull + 16;               //              the unit's last S MMAs have read it
+    constexpr int kSReady = kQFree + 16;              //              S computed
+    constexpr int kPReady = kSReady + 16;             //              first half of P stored
+    constexpr int kP2Ready = kPReady + 16;            //              second half
+    constexpr int kOReady = kP2Ready + 16;            //              O final
+    constexpr int kOFree = kOReady + 16;              //              O read out
+    static_assert(kOFree + 16 <= L::kMisc, "room for the barriers");
+    uint32_t* tmem_slot = (uint32_t*)(smem + L::kMisc);
+    volatile int* const bad_unit = (volatile int*)(smem + L::kMisc + 8);      // 1 + index of the unit the noted rows are of
+    volatile int* const done = (volatile int*)(smem + L::kMisc + 16);         // [query tile] units whose rows are written out
+    int* const bad = (int*)(smem + L::kBad);
+    const WaitCtx wctx{base + L::kMisc + 4, P.status, P.wait_limit_ns};
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        auto init = [&](int off, int n, uint32_t count) {
+            for (int x = 0; x < n; ++x) mbar_init((uint64_t*)(smem + off) + x, count);
+        };
+        init(kFull, L::kStages, 1);
+        init(kEmpty, L::kStages, 2);
+        init(kQFull, 2, 1);
+        init(kQFree, 2, 1);
+        init(kSReady, 2, 1);
+        init(kPReady, 2, 4);
+        init(kP2Ready, 2, 4);
+        init(kOReady, 2, 1);
+        init(kOFree, 2, 4);
+        init(kPassed, L::kStages, 1);
+        *(volatile int*)(smem + L::kMisc + 4) = 0;
+        *bad_unit = 0;
+        done[0] = done[1] = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+#define SA_ARRIVE(OFF, BASE)                       \
+    do {                                           \
+        __syncwarp();                              \
+        if (lane == 0) mbar_arrive<(OFF)>(BASE);   \
+    } while (0)
+
+    if (warp >= 8) {
+        reg_dealloc<kFwdRegsRest>();
+        if (warp == 9) {
+            // ---------------------------------------------------------------- TMA
+            if (lane == 0) {
+                prefetch_tensormap(&map_q);
+                prefetch_tensormap(&map_k);
+                prefetch_tensormap(&map_v);
+                Ring g;
+                uint32_t nq[2] = {0, 0};
+                for (FwdWalk w(P); w.valid(); w.next()) {
+                    const FwdUnit u = w.unit(P);
+                    const int hk = u.h / p.G, nt = u.tiles();
+                    auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head) {
+                        mbar_arrive_expect_tx(bar, L::kTileBytes);
+#pragma unroll
+                        for (int sl = 0; sl < L::kSlabs; ++sl) tma_load_4d(dst + sl * L::kSlab, map, bar, sl * 64, row, head, u.s.b);
+                    };
+                    for (int t = 0; t < nt; ++t)
+#pragma unroll 1
+                        for (int kv = 0; kv < 2; ++kv) {
+                            mbar_wait<kEmpty>(base + 8 * g.s, g.phase ^ 1, wctx, 2 + kv);
+                            load(base + L::kRing + g.s * L::kTileBytes, kv ? &map_v : &map_k, base + kFull + 8 * g.s, u.s.k0 + (u.t0 + t) * kTile, hk);
+                            g.next<L::kStages>();
+                            if (t == 0 && kv == 0)      // behind the first keys: those need not wait for the last unit's Q to be free
+                                for (int r = 0; r < 2; ++r)
+                                    if (u.m(r) > 0) {
+                                        mbar_wait<kQFree>(base + 8 * r, (nq[r] & 1) ^ 1, wctx, 1);
+                                        load(base + L::kQ + r * L::kTileBytes, &map_q, base + kQFull + 8 * r, u.s.q0 + u.i0 + kTile * r, u.h);
+                                        ++nq[r];
+                                    }
+                        }
+                }
+            }
+            __syncwarp();
+        } else if (warp == 8) {
+            // ---------------------------------------------------------------- MMA issuer
+            const uint32_t leader = elect_one();
+            const uint32_t idesc_s = make_idesc(128, kTile, false, false, F16), idesc_o = make_idesc(128, HD, false, true, F16);
+            uint32_t nq[2] = {0, 0}, np[2] = {0, 0};       // units with tiles, tiles so far
+            auto issue_s = [&](int r, int buf, bool last) {
+                const uint32_t da = desc_lo(base + L::kQ + r * L::kTileBytes, 16), db = desc_lo(base + L::kRing + buf * L::kTileBytes, 16);
+                static_for<HD / 16>([&](auto kk_c) {
+                    constexpr int kk = decltype(kk_c)::value, off = ((kk >> 2) * L::kSlab + (kk & 3) * 32) >> 4;
+                    mma_ss_lo<off, off>(leader, tmem + r * kTile, da, db, idesc_s, kk > 0);
+                });
+                tc_commit<kSReady>(leader, base + 8 * r);
+                if (last) tc_commit<kQFree>(leader, base + 8 * r);
+            };
+            // S of a unit's first key tile, for both query tiles
+            auto first_s = [&](const FwdUnit& u, const Ring& g) {
+                if (u.tiles() == 0) return;
+                mbar_wait<kFull>(base + 8 * g.s, g.phase, wctx, 4);
+                for (int r = 0; r < 2; ++r)
+                    if (u.m(r) > 0) {
+                        mbar_wait<kQFull>(base + 8 * r, nq[r] & 1, wctx, 5);
+                        tc_fence_after();
+                        issue_s(r, g.s, u.m(r) == 1);
+                    }
+                tc_commit<kEmpty>(leader, base + 8 * g.s);
+            };
+            Ring g;
+            FwdWalk w(P);
+            FwdUnit u;
+            if (w.valid()) {
+                u = w.unit(P);
+                first_s(u, g);
+            }
+            while (w.valid()) {
+                w.next();
+                FwdUnit un = u;
+                if (w.valid()) un = w.unit(P);
+                const int nt = u.tiles(), guarded = u.first_masked(0);
+#pragma unroll 1
+                for (int t = 0; t < nt; ++t) {
+                    g.next<L::kStages>();
+                    const Ring v = g;
+                    Ring k = g;
+                    k.next<L::kStages>();
+                    const uint32_t db = desc_lo(base + L::kRing + v.s * L::kTileBytes, L::kSlab);
+                    mbar_wait<kFull>(base + 8 * v.s, v.phase, wctx, 6);
+                    if (t >= guarded) mbar_wait<kPassed>(base + 8 * v.s, v.phase, wctx, 7);
+#pragma unroll 1
+                    for (int r = 0; r < 2; ++r) {
+                        if (t >= u.m(r)) continue;
+                        const uint32_t rb = base + 8 * r, tm_s = tmem + r * kTile, tm_o = tmem + 2 * kTile + r * HD;
+                        if (t == 0 && nq[r] > 0) mbar_wait<kOFree>(rb, (nq[r] - 1) & 1, wctx, 8);
+                        mbar_wait<kPReady>(rb, np[r] & 1, wctx, 9);
+                        tc_fence_after();
+                        static_for<4>([&](auto kk_c) {
+                            constexpr int kk = decltype(kk_c)::value;
+                            mma_ts_lo<kk * 8, kk * (2048 >> 4)>(leader, tm_o, tm_s, db, idesc_o, t > 0 || kk > 0);
+                        });
+                        mbar_wait<kP2Ready>(rb, np[r] & 1, wctx, 10);
+                        tc_fence_after();
+                        static_for<4>([&](auto kk_c) {
+                            constexpr int kk = decltype(kk_c)::value + 4;
+                            mma_ts_lo<kk * 8, kk * (2048 >> 4)>(leader, tm_o, tm_s, db, idesc_o, true);
+                        });
+                        ++np[r];
+                        if (t == u.m(r) - 1) {
+                            tc_commit<kOReady>(leader, rb);
+                            ++nq[r];
+                        } else {
+                            mbar_wait<kFull>(base + 8 * k.s, k.phase, wctx, 11);
+                            tc_fence_after();
+                            issue_s(r, k.s, t + 1 == u.m(r) - 1);
+                        }
+                    }
+                    tc_commit<kEmpty>(leader, base + 8 * v.s);
+                    g.next<L::kStages>();
+                    if (t + 1 < nt) tc_commit<kEmpty>(leader, base + 8 * k.s);
+                }
+                u = un;
+                if (w.valid()) first_s(u, g);
+            }
+        } else if (warp == 10) {
+            // ---------------------------------------------------------------- V guard
+            // 8 elements at `at`, of row j and columns d0.., of which this lane's are not all finite if `any`
+            auto note = [&](bool any, uint32_t at, const uint4& x, int j, int d0, uint32_t units) {
+                constexpr uint32_t kExp = F16 ? 0x7c00u : 0x7f80u;
+                if (*bad_unit != (int)units + 1) {
+                    // what is noted now may still be wanted by rows of earlier units: they are written out first
+                    const uint64_t began = globaltimer_ns();
+                    while ((done[0] < (int)units || done[1] < (int)units) && !lds_volatile(wctx.abort_flag) && globaltimer_ns() - began < wctx.limit_ns) {
+                    }
+                    __syncwarp();
+                    for (int d = lane; d < 3 * HD; d += 32) bad[d] = 0x7fffffff;
+                    __threadfence_block();
+                    __syncwarp();
+                    if (lane == 0) *bad_unit = (int)units + 1;
+                    __syncwarp();
+                }
+                if (any) {
+                    uint32_t word[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t h = (word[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+                        if ((~h & kExp) != 0) continue;
+                        atomicMin(&bad[((h & (0x7fffu ^ kExp)) != 0 ? 2 : (int)(h >> 15)) * HD + d0 + e], j);
+                        word[e >> 1] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+                    }
+                    sts128(at, make_uint4(word[0], word[1], word[2], word[3]));
+                }
+                __threadfence_block();
+                __syncwarp();
+            };
+            Ring g;
+            uint32_t units = 0;
+            for (FwdWalk w(P); w.valid(); w.next(), ++units) {
+                const FwdUnit u = w.unit(P);
+                const int nt = u.tiles(), guarded = u.first_masked(0);
+                for (int t = 0; t < nt; ++t) {
+                    // (the guard takes part in every phase of the ring, so that it is never a turn behind or ahead)
+                    mbar_wait<kFull>(base + 8 * g.s, g.phase, wctx, 12);       // K
+                    SA_ARRIVE(kPassed, base + 8 * g.s);
+                    if (lane == 0) mbar_arrive<kEmpty>(base + 8 * g.s);
+                    g.next<L::kStages>();
+                    mbar_wait<kFull>(base + 8 * g.s, g.phase, wctx, 13);       // V
+                    if (t >= guarded) {
+                        const uint32_t tile = base + L::kRing + g.s * L::kTileBytes;
+                        const int j0 = (u.t0 + t) * kTile, rows = u.s.nk - j0;
+                        constexpr uint32_t kExp = F16 ? 0x7c00u : 0x7f80u;
+                        // a lane takes every 32nd 16-byte chunk; the chunks of a slab's 128-byte row are XOR-ed with row & 7
+#pragma unroll 4
+                        for (int c = lane; c < kTile * HD / 8; c += 32) {
+                            const int sl = c / (kTile * 8), row = c / 8 % kTile;
+                            const uint32_t at = tile + c * 16;
+                            const uint4 x = lds128(at);
+                            const uint32_t word[4] = {x.x, x.y, x.z, x.w};
+                            bool any = false;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) any |= (~word[e] & kExp) == 0 || (~word[e] & (kExp << 16)) == 0;
+                            if (row >= rows) sts128(at, make_uint4(0, 0, 0, 0));
+                            any = any && row < rows;
+                            if (__any_sync(0xffffffffu, any)) note(any, at, x, j0 + row, sl * 64 + (((c & 7) ^ (row & 7)) << 3), units);
+                        }
+                        fence_proxy_async_smem();
+                    }
+                    SA_ARRIVE(kPassed, base + 8 * g.s);
+                    if (lane == 0) mbar_arrive<kEmpty>(base + 8 * g.s);
+                    g.next<L::kStages>();
+                }
+            }
+        }
+    } else {
+        // -------------------------------------------------------------------- softmax groups
+        reg_alloc<kFwdRegsSoftmax>();
+        const int r = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(row & ~31) << 16;
+        const uint32_t s_addr = tmem + r * kTile + lanes, o_addr = tmem + 2 * kTile + r * HD + lanes;
+        const uint32_t rb = base + 8 * r;
+        const float c2 = p.scale * kLog2e;
+        uint32_t n = 0, nu = 0, units = 0;
+        for (FwdWalk w(P); w.valid(); w.next(), ++units) {
+            const FwdUnit u = w.unit(P);
+            const int i = u.i0 + kTile * r + row, mt = u.m(r);
+            const int see = i + u.s.off() - u.t0 * kTile;            // last key the row sees, from the first of this share
+            const int masked_from = u.first_masked(r);
+            float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+            for (int t = 0; t < mt; ++t, ++n) {
+                mbar_wait<kSReady>(rb, n & 1, wctx, 14);
+                tc_fence_after();
+                uint32_t v[kTile];
+                {
+                    auto ld = [&](int c) { tmem_ld32(s_addr + 32 * c, reinterpret_cast<uint32_t(&)[32]>(v[32 * c])); };
+                    ld(0);
+                    ld(1);
+                    ld(2);
+                    ld(3);
+                    tmem_wait_ld();
+                }
+                if (t >= masked_from) {
+                    const int hi = see - t * kTile;
+#pragma unroll
+                    for (int c = 0; c < kTile; c += 32) {
+                        const int z = hi - c;
+                        const uint32_t bits = z >= 31 ? ~0u : z < 0 ? 0u : ~0u >> (31 - z);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[c + e] = (bits & (1u << e)) ? v[c + e] : 0xff800000u;
+                    }
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < kTile; e += 8)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) mx[y] = max3(mx[y], __uint_as_float(v[e + y]), __uint_as_float(v[e + 4 + y]));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
+                // The running maximum moves only when it has to; then l and O are scaled down.  (O is at rest: this tile's S
+                // was issued behind the last tile's P V.)
+                float factor = 1.f;
+                if (top > m + kRescaleLog2 || m == -INFINITY) {
+                    if (m > -INFINITY) factor = ex2(m - top);
+                    l *= factor;
+                    m = top;
+                }
+                if (__any_sync(0xffffffffu, factor != 1.f)) {
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HD; c0 += 16) {
+                        uint32_t x[16];
+                        tmem_ld16(o_addr + c0, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * factor);
+                        tmem_st16(o_addr + c0, x);
+                    }
+                }
+                const float nms = m == -INFINITY ? 0.f : -m;
+                const float2 c2v = make_float2(c2, c2), nm = make_float2(nms, nms);
+                float2 ls[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int c = 0; c < kTile; c += 32) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 y = __ffma2_rn(make_float2(__uint_as_float(v[c + e]), __uint_as_float(v[c + e + 1])), c2v, nm);
+                        const float2 pe = make_float2(ex2(y.x), ex2(y.y));
+                        ls[(e >> 1) & 1] = __fadd2_rn(ls[(e >> 1) & 1], pe);
+                        pk[e >> 1] = E::pack(pe.x, pe.y);
+                    }
+                    tmem_st16(s_addr + c / 2, pk);
+                    if (c == kTile / 2 - 32) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        SA_ARRIVE(kPReady, rb);
+                    }
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                SA_ARRIVE(kP2Ready, rb);
+                l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
+            }
+            // ---- the rows of this unit
+            const bool mine = r < P.row_tiles && i < u.s.nq;
+            const int64_t at = ((int64_t)u.s.b * p.H + u.h) * p.Nq + u.s.q0 + i;
+            const int64_t rows = (int64_t)p.B * p.H * p.Nq;
+            const bool none = see < 0 || mt == 0;                    // no key (of this share)
+            if (mt > 0) {
+                mbar_wait<kOReady>(rb, nu & 1, wctx, 15);
+                tc_fence_after();
+                ++nu;
+            }
+            const float inv = none ? 0.f : 1.f / l;
+            const bool noted = *bad_unit == (int)units + 1;
+            __nv_bfloat16* const out = o + u.s.b * p.o.b + (int64_t)(u.s.q0 + i) * p.o.n + u.h * p.o.h;
+            float* const part = P.splits > 1 ? P.part_o + ((int64_t)u.split * rows + at) * HD : nullptr;
+#pragma unroll 1
+            for (int c0 = 0; c0 < HD; c0 += 32) {
+                uint32_t x[32];
+                if (mt > 0) {
+                    tmem_ld32(o_addr + c0, x);
+                    tmem_wait_ld();
+                }
+                if (c0 == HD - 32 && mt > 0) {
+                    tc_fence_before();
+                    SA_ARRIVE(kOFree, rb);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = none ? 0u : __float_as_uint(__uint_as_float(x[e]) * inv);
+                if (noted && !none) {
+                    const int limit = i + u.s.off();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const bool up = bad[c0 + e] <= limit, down = bad[HD + c0 + e] <= limit, nan = bad[2 * HD + c0 + e] <= limit;
+                        if (up || down || nan) x[e] = nan || (up && down) ? 0x7fc00000u : up ? 0x7f800000u : 0xff800000u;
+                    }
+                }
+                if (mine) {
+                    if (part) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + c0 + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8)
+                            *reinterpret_cast<uint4*>(out + c0 + e) =
+                                make_uint4(E::pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), E::pack(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])),
+                                           E::pack(__uint_as_float(x[e + 4]), __uint_as_float(x[e + 5])), E::pack(__uint_as_float(x[e + 6]), __uint_as_float(x[e + 7])));
+                    }
+                }
+            }
+            if (mine) {
+                const float ll = none ? -INFINITY : (m + log2f(l)) * kLn2;
+                if (part) P.part_lse[(int64_t)u.split * rows + at] = ll;
+                else lse[at] = ll;
+            }
+            named_barrier_sync(1 + r, 128);                          // every row has looked at what the guard noted
+            if (row == 0) done[r] = (int)units + 1;
+        }
+    }
+    if (p.cu_q != nullptr) {
+        zero_outside(o, p.o, p.H, HD, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
+        empty_lse_outside(lse, p.H, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+#undef SA_ARRIVE
+
+// Joins the shares of a row: O = sum_s e^(lse_s - lse) O_s, a warp per row and head.  A share without keys has LSE -inf, and
+// its row need not be written.
+template <int HD, bool F16>
+__global__ void __launch_bounds__(256) causal_join_kernel(const CParams p, int splits, const float* __restrict__ part_o, const float* __restrict__ part_lse,
+                                                         __nv_bfloat16* __restrict__ o, float* __restrict__ lse) {
+    using E = ptx::El<F16>;
+    constexpr int kPer = HD / 32;
+    ptx::griddep_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t rows = (int64_t)p.B * p.H * p.Nq, at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (at >= rows) return;
+    const int n = (int)(at % p.Nq), h = (int)(at / p.Nq % p.H), b = (int)(at / p.Nq / p.H);
+    if (p.cu_q != nullptr && (n < p.cu_q[0] || n >= p.cu_q[p.S])) return;       // (written where the shares are)
+    float top = -INFINITY;
+    for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_lse[s * rows + at]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, acc[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+        const float ls = part_lse[s * rows + at];
+        if (ls == -INFINITY) continue;
+        const float w = expf(ls - base);
+        sum += w;
+        const float* src = part_o + (s * rows + at) * HD + kPer * lane;
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) {
+            const float2 x = *reinterpret_cast<const float2*>(src + e);
+            acc[e] = fmaf(w, x.x, acc[e]);
+            acc[e + 1] = fmaf(w, x.y, acc[e + 1]);
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    __nv_bfloat16* dst = o + b * p.o.b + (int64_t)n * p.o.n + h * p.o.h + kPer * lane;
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = E::pack(acc[e] * inv, acc[e + 1] * inv);
+    if (lane == 0) lse[at] = sum == 0.f ? -INFINITY : top + logf(sum);
+}
+
+// Launches a kernel that may start while the one before it in the stream still runs (it waits for it by itself).
+template <typename... Args, typename... Given>
+cudaError_t launch_behind(void (*kern)(Args...), unsigned grid, unsigned block, int smem, cudaStream_t st, Given... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, Args(args)...);
+}
+
+template <int HD>
+int launch_join(const CParams& p, bool f16, int splits, const float* part_o, const float* part_lse, void* o, float* lse, cudaStream_t st) {
+    const unsigned grid = (unsigned)(((int64_t)p.B * p.H * p.Nq + 7) / 8);
+    const cudaError_t e = f16 ? launch_behind(causal_join_kernel<HD, true>, grid, 256, 0, st, p, splits, part_o, part_lse, (__nv_bfloat16*)o, lse)
+                              : launch_behind(causal_join_kernel<HD, false>, grid, 256, 0, st, p, splits, part_o, part_lse, (__nv_bfloat16*)o, lse);
+    host::count_launches(1);
+    return e == cudaSuccess ? SA_OK : SA_ERR_LAUNCH;
+}
+
+// How a call is cut up, and its workspace.
+struct FwdPlan {
+    int row_tiles, splits;
+    int64_t items;                    // at most
+    size_t list, part_o, part_lse, bytes;
+};
+inline FwdPlan plan_fwd(const CParams& c) {
+    FwdPlan f{};
+    const int sms = host::sm_count();
+    auto items = [&](int tiles) {
+        return c.cu_q != nullptr ? list_capacity(c.Nq, kTile * tiles, c.S) : (int64_t)ceil_div(c.Nq, kTile * tiles) * c.S;
+    };
+    // Pairs of query tiles that do not fill the multiprocessors are taken apart.
+    f.row_tiles = items(2) * c.H > sms ? 2 : 1;
+    f.items = items(f.row_tiles);
+    // Shares of the keys, where there are few units: rounds of blocks times the key tiles of the longest unit, with two more
+    // for what a unit costs besides and four for joining, in units of a key tile's time (about 1.5 us).
+    const int64_t units = f.items * c.H;
+    const int tiles = ceil_div(c.max_k, kTile);
+    f.splits = 1;
+    int64_t best = (units + sms - 1) / sms * (tiles + 2);
+    for (int s = 2; s <= 32 && 2 * s <= tiles && units * (s - 1) < 2 * sms; ++s) {
+        const int64_t cost = (units * s + sms - 1) / sms * (ceil_div(tiles, s) + 2) + 4;
+        if (cost < best) {
+            best = cost;
+            f.splits = s;
+        }
+    }
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };
+    f.list = take(c.cu_q != nullptr ? list_bytes(f.items) : 0);
+    const size_t rows = (size_t)c.B * c.H * c.Nq;
+    f.part_o = take(f.splits > 1 ? (size_t)f.splits * rows * c.D * 4 : 0);
+    f.part_lse = take(f.splits > 1 ? (size_t)f.splits * rows * 4 : 0);
+    f.bytes = at;
+    return f;
+}
+
+template <int HD, bool F16>
+int launch_fwd_tc(const CParams& c, const void* q, const void* k, const void* v, void* o, float* lse, uint8_t* ws, DeviceStatus* status, cudaStream_t st) {
+    const FwdPlan f = plan_fwd(c);
+    if (f.items * c.H * f.splits > 0x3fffffff) return SA_ERR_UNSUPPORTED;
+    CUtensorMap mq, mk, mv;
+    if (!host::make_map(&mq, q, c.B, c.Nq, c.H, HD, c.q, kTile, F16) || !host::make_map(&mk, k, c.B, c.Nk, c.Hkv, HD, c.k, kTile, F16) ||
+        !host::make_map(&mv, v, c.B, c.Nk, c.Hkv, HD, c.v, kTile, F16))
+        return SA_ERR_BAD_STRIDE;
+    FwdParams P{};
+    P.c = c;
+    P.row_tiles = f.row_tiles;
+    P.splits = f.splits;
+    P.part_o = reinterpret_cast<float*>(ws + f.part_o);
+    P.part_lse = reinterpret_cast<float*>(ws + f.part_lse);
+    P.status = status;
+    P.wait_limit_ns = host::wait_limit_ns();
+    P.work.tiles = ceil_div(c.Nq, kTile * f.row_tiles);
+    P.work.S = c.S;
+    P.work.descending = 1;
+    auto kern = causal_fwd_tc_kernel<HD, F16>;
+    if (!allow_dynamic_smem((const void*)kern, FwdLayout<HD>::kBytes)) return SA_ERR_LAUNCH;
+    if (c.cu_q != nullptr) {
+        PlanParams plan{};
+        plan.list[0] = reinterpret_cast<ListHead*>(ws + f.list);
+        plan.rows[0] = kTile * f.row_tiles;
+        plan.capacity[0] = (int)f.items;
+        P.work.head = plan.list[0];
+        causal_plan_kernel<<<1, 1024, 0, st>>>(c, plan);
+        host::count_launches(1);
+    }
+    const int64_t units = f.items * c.H * f.splits;
+    const unsigned grid = (unsigned)(units < host::sm_count() ? units : host::sm_count());
+    kern<<<grid, kFwdThreads, FwdLayout<HD>::kBytes, st>>>(P, mq, mk, mv, (__nv_bfloat16*)o, lse);
+    host::count_launches(1);
+    if (cudaGetLastError() != cudaSuccess) return SA_ERR_LAUNCH;
+    return f.splits > 1 ? launch_join<HD>(c, F16, f.splits, P.part_o, P.part_lse, o, lse, st) : SA_OK;
+}
+
+}  // namespace causal
+}  // namespace sa

@@ -1,0 +1,131 @@
+// What the tensor-core causal attention kernels share: units of work, their order, the plan of a packed batch.
+#pragma once
+
+#include "sa_causal.cuh"
+#include "sa_ptx.cuh"
+
+namespace sa {
+namespace causal {
+
+constexpr int kTile = 128;            // rows of a query tile = lanes of tensor memory, and keys of a key tile
+
+// One entry of a packed batch's list of work: a tile of a sequence.
+struct alignas(32) Item {
+    int q0, nq, k0, nk;
+    int tile;
+    int pad[3];
+};
+struct alignas(32) ListHead {
+    int count;
+    int pad[7];
+};
+
+// Work of one kernel: tiles of `rows` queries (or keys), the most expensive first, so that the blocks that end last hold short
+// ones.  Without a list (batched tensors) tile and sequence follow from the index.
+struct WorkList {
+    const ListHead* head;             // NULL: no list; items follow the head
+    int tiles, S;                     // without a list: tiles per sequence, sequences
+    int descending;                   // without a list: whether later tiles are the more expensive ones
+};
+
+__device__ __forceinline__ int list_count(const WorkList& w) { return w.head ? w.head->count : w.tiles * w.S; }
+
+__device__ __forceinline__ void list_item(const CParams& p, const WorkList& w, int i, Seq& s, int& tile) {
+    if (w.head) {
+        const Item* e = reinterpret_cast<const Item*>(w.head + 1) + i;
+        const int4 a = *reinterpret_cast<const int4*>(e);
+        // (clipped again: starts that decrease may leave entries of the list unwritten)
+        s.b = 0;
+        s.q0 = min(max(a.x, 0), p.Nq);
+        s.nq = min(max(a.y, 0), p.Nq - s.q0);
+        s.k0 = min(max(a.z, 0), p.Nk);
+        s.nk = min(max(a.w, 0), p.Nk - s.k0);
+        tile = min(max(e->tile, 0), 1 << 23);
+    } else {
+        tile = i / w.S;
+        s.b = i - tile * w.S;
+        s.q0 = s.k0 = 0;
+        s.nq = p.Nq;
+        s.nk = p.Nk;
+        if (w.descending) tile = w.tiles - 1 - tile;
+    }
+}
+
+// Key tiles that query tiles of rows [i0, i0 + rows) see; query tiles that see a key of the tile at j0.
+__host__ __device__ inline int key_tiles(int i0, int rows, int nq, int nk) {
+    if (i0 >= nq) return 0;
+    const int last = i0 + rows < nq ? i0 + rows : nq;
+    const int seen = last + nk - nq;
+    return seen > 0 ? (seen + kTile - 1) / kTile : 0;
+}
+__host__ __device__ inline int first_query(int j0, int nq, int nk) {       // a multiple of the tile
+    const int i = j0 - (nk - nq);
+    return i > 0 ? i / kTile * kTile : 0;
+}
+
+// The lists of a packed batch, a block for each: tiles of `rows[list]` queries (keys where by_key[list]), sorted by cost in one
+// counting pass.  Items of equal cost come in any order: it decides where they run, not what they compute.
+struct PlanParams {
+    ListHead* list[2];
+    int rows[2], by_key[2];
+    int capacity[2];                  // tiles of sequences that do not overlap (starts that decrease: the rest is left out)
+};
+constexpr int kPlanBins = 1024;
+__global__ void __launch_bounds__(1024) causal_plan_kernel(const CParams p, const PlanParams plan) {
+    __shared__ int bins[kPlanBins], warp_sums[32];
+    ListHead* const head = plan.list[blockIdx.x];
+    const int rows = plan.rows[blockIdx.x], by_key = plan.by_key[blockIdx.x];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    bins[t] = 0;
+    __syncthreads();
+    auto each = [&](auto&& f) {
+        for (int s = warp; s < p.S; s += 32) {
+            const Seq q = seq_of(p, s);
+            const int n = by_key ? q.nk : q.nq;
+            for (int tile = lane; tile * rows < n; tile += 32) {
+                const int cost = by_key ? max(ceil_div(q.nq - first_query(tile * rows, q.nq, q.nk), kTile), 0) : key_tiles(tile * rows, rows, q.nq, q.nk);
+                f(q, tile, kPlanBins - 1 - min(cost, kPlanBins - 1));
+            }
+        }
+    };
+    each([&](const Seq&, int, int bin) { atomicAdd(&bins[bin], 1); });
+    __syncthreads();
+    // exclusive prefix sum over the bins
+    int v = bins[t], x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        int w = warp_sums[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+        }
+        warp_sums[lane] = w;
+    }
+    __syncthreads();
+    x += (warp ? warp_sums[warp - 1] : 0) - v;
+    if (t == 1023) head->count = min(max(x + v, 0), plan.capacity[blockIdx.x]);
+    bins[t] = x;
+    __syncthreads();
+    Item* const items = reinterpret_cast<Item*>(head + 1);
+    each([&](const Seq& q, int tile, int bin) {
+        const int at = atomicAdd(&bins[bin], 1);
+        if ((unsigned)at >= (unsigned)plan.capacity[blockIdx.x]) return;
+        Item* e = items + at;
+        *reinterpret_cast<int4*>(e) = make_int4(q.q0, q.nq, q.k0, q.nk);
+        e->tile = tile;
+    });
+}
+
+// Tiles of S sequences that share `rows` rows, at most, and the bytes of a list of so many.
+inline int64_t list_capacity(int rows, int tile, int S) { return (int64_t)rows / tile + S; }
+inline size_t list_bytes(int64_t items) { return (size_t)(sizeof(ListHead) + items * sizeof(Item) + 255) / 256 * 256; }
+
+}  // namespace causal
+}  // namespace sa
