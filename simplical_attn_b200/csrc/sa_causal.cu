@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "sa_causal.cuh"
+#include "sa_causal_bwd.cuh"
 #include "sa_causal_fwd.cuh"
 #include "sa_causal_general.cuh"
 
@@ -44,7 +45,6 @@ CParams make_params(const sa_causal_params* p, const int32_t* cu_q, const int32_
 
 // Whether the tensor-core kernels cover the problem (pointers and what a tensor map can hold are looked at in the call).
 bool tc_ok(const sa_causal_params* p, bool backward) {
-    if (backward) return false;
     if (p->dtype == SA_F32 || (p->D != 64 && p->D != 128)) return false;
     if (!(p->scale > 0.f)) return false;            // the row maximum is taken before scaling
     const CParams c = make_params(p, nullptr, nullptr);
@@ -99,7 +99,8 @@ size_t sa_causal_forward_workspace_size(const sa_causal_params* p) {
 size_t sa_causal_backward_workspace_size(const sa_causal_params* p) {
     using namespace sa::causal;
     if (validate(p) != SA_OK) return 0;
-    return delta_bytes(p);
+    if (resolve(p, true) != SA_ALGO_TCGEN05) return delta_bytes(p);
+    return plan_bwd(planned(p)).bytes;
 }
 
 int sa_causal_resolve(const sa_causal_params* p, int backward) {
@@ -147,6 +148,18 @@ int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, 
     const CParams c = make_params(p, p->sequences > 0 ? cu_q : nullptr, p->sequences > 0 ? cu_k : nullptr);
     float* delta = static_cast<float*>(workspace);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (algo == SA_ALGO_TCGEN05) {
+        if (sa::host::cc_major() != 10) return SA_ERR_NOT_SM100;
+        rc = SA_ERR_BAD_STRIDE;
+        bool aligned = true;
+        for (const void* x : {q, k, v, o, d_o, (const void*)dq, (const void*)dk, (const void*)dv}) aligned = aligned && sa::host::aligned16(x);
+        if (aligned)
+            rc = dispatch_tc(p, [&](auto d, auto f16) {
+                return launch_bwd_tc<decltype(d)::value, decltype(f16)::value>(c, q, k, v, o, lse, d_o, dq, dk, dv, static_cast<uint8_t*>(workspace),
+                                                                             static_cast<sa::DeviceStatus*>(status), st);
+            });
+        if (rc != SA_ERR_BAD_STRIDE || p->algo == SA_ALGO_TCGEN05) return rc;
+    }
     return dispatch_general(p->dtype, p->D, [&](auto t, auto d) {
         return launch_general_bwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, lse, d_o, dq, dk, dv, delta, st);
     });
