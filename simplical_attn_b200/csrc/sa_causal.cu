@@ -6,6 +6,7 @@
 
 #include "sa_causal.cuh"
 #include "sa_causal_bwd.cuh"
+#include "sa_causal_few.cuh"
 #include "sa_causal_fwd.cuh"
 #include "sa_causal_general.cuh"
 
@@ -58,8 +59,10 @@ bool tc_ok(const sa_causal_params* p, bool backward) {
 
 int resolve(const sa_causal_params* p, bool backward) {
     const bool ok = p->algo != SA_ALGO_GENERAL && tc_ok(p, backward);
-    if (p->algo == SA_ALGO_TCGEN05 && !ok) return -SA_ERR_UNSUPPORTED;
-    return ok ? SA_ALGO_TCGEN05 : SA_ALGO_GENERAL;
+    if (p->algo == SA_ALGO_TCGEN05) return ok ? SA_ALGO_TCGEN05 : -SA_ERR_UNSUPPORTED;
+    if (!ok) return SA_ALGO_GENERAL;
+    const CParams c = make_params(p, nullptr, nullptr);
+    return !backward && (int64_t)c.max_q * c.G <= kFewRowsMost ? SA_CAUSAL_FEW_ROWS : SA_ALGO_TCGEN05;
 }
 
 // (a plan only asks whether there are starts)
@@ -92,8 +95,9 @@ extern "C" {
 
 size_t sa_causal_forward_workspace_size(const sa_causal_params* p) {
     using namespace sa::causal;
-    if (validate(p) != SA_OK || resolve(p, false) != SA_ALGO_TCGEN05) return 0;
-    return plan_fwd(planned(p)).bytes;
+    if (validate(p) != SA_OK) return 0;
+    const int algo = resolve(p, false);
+    return algo == SA_ALGO_TCGEN05 ? plan_fwd(planned(p)).bytes : algo == SA_CAUSAL_FEW_ROWS ? plan_few(planned(p)).bytes : 0;
 }
 
 size_t sa_causal_backward_workspace_size(const sa_causal_params* p) {
@@ -120,11 +124,13 @@ int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, c
     if (algo < 0) return -algo;
     const CParams c = make_params(p, p->sequences > 0 ? cu_q : nullptr, p->sequences > 0 ? cu_k : nullptr);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (algo == SA_ALGO_TCGEN05) {
+    if (algo != SA_ALGO_GENERAL) {
         if (sa::host::cc_major() != 10) return SA_ERR_NOT_SM100;
         rc = SA_ERR_BAD_STRIDE;
         if (sa::host::aligned16(q) && sa::host::aligned16(k) && sa::host::aligned16(v) && sa::host::aligned16(o))
             rc = dispatch_tc(p, [&](auto d, auto f16) {
+                if (algo == SA_CAUSAL_FEW_ROWS)
+                    return launch_few<decltype(d)::value, decltype(f16)::value>(c, q, k, v, o, lse, static_cast<uint8_t*>(workspace), st);
                 return launch_fwd_tc<decltype(d)::value, decltype(f16)::value>(c, q, k, v, o, lse, static_cast<uint8_t*>(workspace),
                                                                              static_cast<sa::DeviceStatus*>(status), st);
             });

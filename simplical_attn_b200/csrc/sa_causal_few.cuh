@@ -1,0 +1,394 @@
+// Causal attention of a few queries over many keys (single tokens, a handful of drafted ones), bf16 / fp16, head dim 64 and 128.
+//
+// K and V are read once and little is computed with them: HBM bandwidth bounds it, latency where they are short.  The rows of
+// a block are the queries of all heads that share a KV head (query i, head g of the group: row i G + g), 16 or 32 of them, so a
+// key is read once for the group.  The keys of a sequence are cut into shares, a block each, joined by causal_join_kernel.
+//
+// The products are 16 x 8 x 16 register MMAs (mma.sync): tcgen05 works on 128 rows, of which these calls would fill 16.  A warp
+// has its own 16 of every 64 keys, copied by its own asynchronous copies into its own part of shared memory, with its own
+// running maximum, sum and rows of O: warps wait for nobody until they are merged at the end.
+#pragma once
+
+#include "sa_causal_fwd.cuh"
+
+namespace sa {
+namespace causal {
+
+constexpr int kFewThreads = 128;
+constexpr int kFewKeys = 64;              // keys of a step of the block: 16 per warp
+constexpr int kFewRowsMost = 32;          // rows (queries times heads of a group) that these kernels are taken for
+
+struct FewParams {
+    CParams c;
+    int shares, row_blocks;               // of a sequence's keys, and of its rows
+    float* part_o;                        // shares > 1: as in FwdParams
+    float* part_lse;
+};
+
+template <int HD, int MT>
+struct FewLayout {
+    static constexpr int kStages = 3;
+    static constexpr int kHalf = 16 * HD * 2;                       // 16 rows of K, or of V
+    static constexpr int kWarp = kStages * 2 * kHalf;
+    static constexpr int kQ = 16 * MT * HD * 2;
+    static constexpr int kStats = 2 * 4 * 16 * MT * 4;              // m, l: [warp][row]
+    static constexpr int kBytes = kQ + kStats + 4 * kWarp;
+    static_assert(4 * 16 * MT * HD * 4 <= 4 * kWarp, "the rows of the warps are merged where K and V were");
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Whether one of two packed elements is infinite or NaN.
+template <bool F16>
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+    constexpr uint32_t kExp = F16 ? 0x7c00u : 0x7f80u;
+    return (~w & kExp) == 0 || (~w & (kExp << 16)) == 0;
+}
+
+template <int HD, bool F16, int MT>
+__global__ void __launch_bounds__(kFewThreads, MT == 1 ? 2 : 2)
+causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ k,
+                  const __nv_bfloat16* __restrict__ v, __nv_bfloat16* __restrict__ o, float* __restrict__ lse) {
+    using L = FewLayout<HD, MT>;
+    using E = ptx::El<F16>;
+    constexpr int kChunks = HD / 8;               // 16-byte chunks of a row
+    extern __shared__ uint4 smem16[];
+    uint8_t* const smem = reinterpret_cast<uint8_t*>(smem16);
+    const CParams& p = P.c;
+    ptx::griddep_launch();                        // (the joining kernel waits for this one's end by itself)
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // the shares of a sequence and head lie side by side: what runs at a time spreads over sequences of all lengths
+    int x = blockIdx.x;
+    const int share = x % P.shares;
+    x /= P.shares;
+    const int rb0 = x % P.row_blocks;
+    x /= P.row_blocks;
+    const int hk = x % p.Hkv;
+    const Seq s = seq_of(p, x / p.Hkv);
+    const int R = s.nq * p.G;
+    const int64_t rows_all = (int64_t)p.B * p.H * p.Nq;
+    // whole steps of keys per share, as many as the sequence needs
+    const int steps_all = (s.nk + kFewKeys - 1) / kFewKeys, per = (steps_all + P.shares - 1) / P.shares;
+    const int c0 = min(share * per * kFewKeys, s.nk), c1 = min(c0 + per * kFewKeys, s.nk);
+    const int steps = (c1 - c0 + kFewKeys - 1) / kFewKeys;
+
+    const uint32_t q_st = ptx::smem_u32(smem), w_st = q_st + L::kQ + L::kStats + warp * L::kWarp;
+    float* const stat_m = reinterpret_cast<float*>(smem + L::kQ);
+    float* const stat_l = stat_m + 4 * 16 * MT;
+    const __nv_bfloat16* const kh = k + s.b * p.k.b + (int64_t)s.k0 * p.k.n + hk * p.k.h;
+    const __nv_bfloat16* const vh = v + s.b * p.v.b + (int64_t)s.k0 * p.v.n + hk * p.v.h;
+    const float c2 = p.scale * kLog2e;
+
+    for (int rb = rb0; rb * 16 * MT < R; rb += P.row_blocks) {
+        const int r0 = rb * 16 * MT;
+        auto load = [&](int t) {
+            if (t < steps) {
+                const int j0 = c0 + t * kFewKeys + warp * 16;
+                const uint32_t st = w_st + (t % L::kStages) * 2 * L::kHalf;
+#pragma unroll
+                for (int e = 0; e < 16 * kChunks / 32; ++e) {
+                    const int c = lane + 32 * e, row = c / kChunks, ch = c % kChunks, j = j0 + row;
+                    const uint32_t at = st + row * HD * 2 + ((ch ^ (row & 7)) << 4);
+                    const bool in = j < c1;
+                    const int64_t jj = in ? j : c0;
+                    cp16(at, kh + jj * p.k.n + ch * 8, in);               // rows behind the share: zeros
+                    cp16(at + L::kHalf, vh + jj * p.v.n + ch * 8, in);
+                }
+            }
+            cp_commit();
+        };
+        if (steps > 0) {
+#pragma unroll
+            for (int t = 0; t < L::kStages - 1; ++t) load(t);
+        }
+        // rows of Q: zeros where there are none
+        for (int c = tid; c < 16 * MT * kChunks; c += kFewThreads) {
+            const int row = c / kChunks, ch = c % kChunks, rho = r0 + row;
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (rho < R) {
+                const int i = rho / p.G, g = rho - i * p.G;
+                w = *reinterpret_cast<const uint4*>(q + s.b * p.q.b + (int64_t)(s.q0 + i) * p.q.n + (hk * p.G + g) * p.q.h + ch * 8);
+            }
+            *reinterpret_cast<uint4*>(smem + row * HD * 2 + ((ch ^ (row & 7)) << 4)) = w;
+        }
+        __syncthreads();
+        // this thread's rows (lane / 4 and 8 further down, of every 16): last key seen, running maximum and sum
+        int last[2 * MT];
+        float m[2 * MT], l[2 * MT], acc[MT][HD / 8][4];
+#pragma unroll
+        for (int y = 0; y < 2 * MT; ++y) {
+            const int rho = r0 + 8 * y + (lane >> 2);
+            last[y] = rho < R ? min(rho / p.G + s.off(), c1 - 1) : -1;
+            m[y] = -INFINITY;
+            l[y] = 0.f;
+        }
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[a][d][e] = 0.f;
+        const int first_last = r0 / p.G + s.off();                 // last key the block's first row sees
+
+#pragma unroll 1
+        for (int t = 0; t < steps; ++t) {
+            cp_wait<L::kStages - 2>();
+            __syncwarp();
+            load(t + L::kStages - 1);              // (into the buffer of step t - 1, which every lane has left)
+            const int j0 = c0 + t * kFewKeys + warp * 16;
+            if (j0 >= c1) continue;
+            const uint32_t st = w_st + (t % L::kStages) * 2 * L::kHalf;
+            const bool masked = j0 + 15 > min(first_last, c1 - 1);
+            uint32_t pa[MT][4];
+            float sc[MT][2][4];
+#pragma unroll
+            for (int a = 0; a < MT; ++a)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sc[a][e >> 2][e & 3] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                uint32_t kb[4];
+                {
+                    const int row = (lane >> 4) * 8 + (lane & 7), ch = 2 * kk + ((lane >> 3) & 1);
+                    ldm4(kb, st + row * HD * 2 + ((ch ^ (row & 7)) << 4));
+                }
+#pragma unroll
+                for (int a = 0; a < MT; ++a) {
+                    uint32_t qa[4];
+                    const int row = 16 * a + (lane & 15), ch = 2 * kk + (lane >> 4);
+                    ldm4(qa, q_st + row * HD * 2 + ((ch ^ (row & 7)) << 4));
+                    mma16816<F16>(sc[a][0], qa, kb[0], kb[1]);
+                    mma16816<F16>(sc[a][1], qa, kb[2], kb[3]);
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < MT; ++a) {
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int hf = (e >> 1) & 1, j = j0 + 8 * (e >> 2) + 2 * (lane & 3) + (e & 1);
+                    float& y = sc[a][e >> 2][e & 3];
+                    y = !masked || j <= last[2 * a + hf] ? y * c2 : -INFINITY;
+                    top[hf] = fmaxf(top[hf], y);
+                }
+                float f[2];
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    float& mm = m[2 * a + hf];
+                    top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 1));
+                    top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 2));
+                    f[hf] = 1.f;
+                    if (top[hf] > mm + kRescaleLog2 || mm == -INFINITY) {
+                        if (mm > -INFINITY) f[hf] = ptx::ex2(mm - top[hf]);
+                        mm = top[hf];
+                    }
+                    l[2 * a + hf] *= f[hf];
+                }
+                if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+                    for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[a][d][e] *= f[e >> 1];
+                }
+                const float b0 = m[2 * a] == -INFINITY ? 0.f : m[2 * a], b1 = m[2 * a + 1] == -INFINITY ? 0.f : m[2 * a + 1];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float& y = sc[a][e >> 2][e & 3];
+                    y = ptx::ex2(y - ((e >> 1) & 1 ? b1 : b0));
+                    l[2 * a + ((e >> 1) & 1)] += y;
+                }
+                // the accumulators' layout is that of the A operand of the next product
+                pa[a][0] = E::pack(sc[a][0][0], sc[a][0][1]);
+                pa[a][1] = E::pack(sc[a][0][2], sc[a][0][3]);
+                pa[a][2] = E::pack(sc[a][1][0], sc[a][1][1]);
+                pa[a][3] = E::pack(sc[a][1][2], sc[a][1][3]);
+            }
+            bool odd = false;                      // a V element that is not finite, under a mask
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 16 * kChunks / 32; ++e) {
+                    const uint4 w = ptx::lds128(st + L::kHalf + (lane + 32 * e) * 16);
+                    odd |= not_finite2<F16>(w.x) || not_finite2<F16>(w.y) || not_finite2<F16>(w.z) || not_finite2<F16>(w.w);
+                }
+                odd = __any_sync(0xffffffffu, odd);
+            }
+            if (!odd) {
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) {
+                    uint32_t vb[4];
+                    const int row = ((lane >> 3) & 1) * 8 + (lane & 7), ch = 2 * d + (lane >> 4);
+                    ldm4t(vb, st + L::kHalf + row * HD * 2 + ((ch ^ (row & 7)) << 4));
+#pragma unroll
+                    for (int a = 0; a < MT; ++a) {
+                        mma16816<F16>(acc[a][2 * d], pa[a], vb[0], vb[1]);
+                        mma16816<F16>(acc[a][2 * d + 1], pa[a], vb[2], vb[3]);
+                    }
+                }
+            } else {
+                // key by key, only into rows that see it: a masked zero times it would not be zero
+#pragma unroll 1
+                for (int j = 0; j < 16; ++j)
+#pragma unroll
+                    for (int a = 0; a < MT; ++a) {
+                        const int from = (lane & ~3) | ((j & 7) >> 1);
+                        const uint32_t w0 = __shfl_sync(0xffffffffu, j < 8 ? pa[a][0] : pa[a][2], from), w1 = __shfl_sync(0xffffffffu, j < 8 ? pa[a][1] : pa[a][3], from);
+                        const float p0 = j & 1 ? E::hi(w0) : E::lo(w0), p1 = j & 1 ? E::hi(w1) : E::lo(w1);
+                        const bool see0 = j0 + j <= last[2 * a], see1 = j0 + j <= last[2 * a + 1];
+#pragma unroll
+                        for (int d = 0; d < HD / 8; ++d) {
+                            const uint32_t w = ptx::lds32(st + L::kHalf + j * HD * 2 + ((d ^ (j & 7)) << 4) + (lane & 3) * 4);
+                            if (see0) {
+                                acc[a][d][0] = fmaf(p0, E::lo(w), acc[a][d][0]);
+                                acc[a][d][1] = fmaf(p0, E::hi(w), acc[a][d][1]);
+                            }
+                            if (see1) {
+                                acc[a][d][2] = fmaf(p1, E::lo(w), acc[a][d][2]);
+                                acc[a][d][3] = fmaf(p1, E::hi(w), acc[a][d][3]);
+                            }
+                        }
+                    }
+            }
+        }
+        cp_wait<0>();
+        // ---- merge the warps
+#pragma unroll
+        for (int y = 0; y < 2 * MT; ++y) {
+            l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
+            l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+            if ((lane & 3) == 0) {
+                stat_m[warp * 16 * MT + 8 * y + (lane >> 2)] = m[y];
+                stat_l[warp * 16 * MT + 8 * y + (lane >> 2)] = l[y];
+            }
+        }
+        __syncthreads();                           // (every warp has left its K and V)
+        float* const merge = reinterpret_cast<float*>(smem + L::kQ + L::kStats);
+        {
+            float* const mine = merge + warp * 16 * MT * HD;
+#pragma unroll
+            for (int a = 0; a < MT; ++a)
+#pragma unroll
+                for (int d = 0; d < HD / 8; ++d) {
+                    const int r = 16 * a + (lane >> 2), col = 8 * d + 2 * (lane & 3);
+                    *reinterpret_cast<float2*>(mine + r * HD + (col ^ ((r & 3) << 3))) = make_float2(acc[a][d][0], acc[a][d][1]);
+                    *reinterpret_cast<float2*>(mine + (r + 8) * HD + (col ^ ((r & 3) << 3))) = make_float2(acc[a][d][2], acc[a][d][3]);
+                }
+        }
+        __syncthreads();
+        for (int c = tid; c < 16 * MT * (HD / 4); c += kFewThreads) {
+            const int r = c / (HD / 4), d = c % (HD / 4) * 4, rho = r0 + r;
+            if (rho >= R) continue;
+            float top = -INFINITY, w[4], sum = 0.f;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) top = fmaxf(top, stat_m[y * 16 * MT + r]);
+            const float b = top == -INFINITY ? 0.f : top;
+            float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                w[y] = ptx::ex2(stat_m[y * 16 * MT + r] - b);
+                sum += w[y] * stat_l[y * 16 * MT + r];
+                const float4 z = *reinterpret_cast<const float4*>(merge + (y * 16 * MT + r) * HD + (d ^ ((r & 3) << 3)));
+                // (a warp that has seen no key of the row holds zeros)
+                t.x = fmaf(w[y], z.x, t.x);
+                t.y = fmaf(w[y], z.y, t.y);
+                t.z = fmaf(w[y], z.z, t.z);
+                t.w = fmaf(w[y], z.w, t.w);
+            }
+            const int i = rho / p.G, h = hk * p.G + rho - i * p.G;
+            const bool none = min(i + s.off(), c1 - 1) < c0;
+            const float inv = none ? 0.f : 1.f / sum;
+            const int64_t at = ((int64_t)s.b * p.H + h) * p.Nq + s.q0 + i;
+            const float ll = none ? -INFINITY : (top + log2f(sum)) * kLn2;
+            if (none) t = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (P.shares > 1) {
+                if (!none) *reinterpret_cast<float4*>(P.part_o + (share * rows_all + at) * HD + d) = make_float4(t.x * inv, t.y * inv, t.z * inv, t.w * inv);
+                if (d == 0) P.part_lse[share * rows_all + at] = ll;
+            } else {
+                *reinterpret_cast<uint2*>(o + s.b * p.o.b + (int64_t)(s.q0 + i) * p.o.n + h * p.o.h + d) =
+                    make_uint2(E::pack(t.x * inv, t.y * inv), E::pack(t.z * inv, t.w * inv));
+                if (d == 0) lse[at] = ll;
+            }
+        }
+        __syncthreads();
+    }
+    if (p.cu_q != nullptr) {
+        zero_outside(o, p.o, p.H, HD, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
+        empty_lse_outside(lse, p.H, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
+    }
+}
+
+struct FewPlan {
+    int mt, shares, row_blocks;
+    size_t part_o, part_lse, bytes;
+};
+inline FewPlan plan_few(const CParams& c) {
+    FewPlan f{};
+    const int rows = (int)((int64_t)c.max_q * c.G < kFewRowsMost ? c.max_q * c.G : kFewRowsMost);
+    f.mt = rows > 16 ? 2 : 1;
+    f.row_blocks = ceil_div(rows, 16 * f.mt);
+    // Shares of at least four steps, enough for three rounds of blocks over the multiprocessors (two at a time each): packed
+    // sequences are shorter than the longest, so theirs are cut by the mean.
+    const int64_t blocks = (int64_t)c.S * c.Hkv * f.row_blocks, want = 6 * host::sm_count();
+    const int64_t mean = c.cu_q != nullptr && c.Nk / c.S < c.max_k ? (c.Nk / c.S > 0 ? c.Nk / c.S : 1) : c.max_k;
+    int64_t shares = (want * c.max_k / mean + blocks - 1) / blocks;
+    const int64_t most = ceil_div(c.max_k, 4 * kFewKeys);
+    if (shares > most) shares = most;
+    if (shares > 256) shares = 256;
+    f.shares = shares < 1 ? 1 : (int)shares;
+    const size_t all = (size_t)c.B * c.H * c.Nq;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };
+    f.part_o = take(f.shares > 1 ? (size_t)f.shares * all * c.D * 4 : 0);
+    f.part_lse = take(f.shares > 1 ? (size_t)f.shares * all * 4 : 0);
+    f.bytes = at;
+    return f;
+}
+
+template <int HD, bool F16>
+int launch_few(const CParams& c, const void* q, const void* k, const void* v, void* o, float* lse, uint8_t* ws, cudaStream_t st) {
+    const FewPlan f = plan_few(c);
+    const int64_t grid = (int64_t)c.S * c.Hkv * f.row_blocks * f.shares;
+    if (grid > 0x7fffffff) return SA_ERR_UNSUPPORTED;
+    FewParams P{};
+    P.c = c;
+    P.shares = f.shares;
+    P.row_blocks = f.row_blocks;
+    P.part_o = reinterpret_cast<float*>(ws + f.part_o);
+    P.part_lse = reinterpret_cast<float*>(ws + f.part_lse);
+    auto go = [&](auto mt) {
+        constexpr int MT = decltype(mt)::value;
+        auto kern = causal_few_kernel<HD, F16, MT>;
+        if (!allow_dynamic_smem((const void*)kern, FewLayout<HD, MT>::kBytes)) return SA_ERR_LAUNCH;
+        kern<<<(unsigned)grid, kFewThreads, FewLayout<HD, MT>::kBytes, st>>>(P, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v,
+                                                                             (__nv_bfloat16*)o, lse);
+        host::count_launches(1);
+        return cudaGetLastError() == cudaSuccess ? SA_OK : SA_ERR_LAUNCH;
+    };
+    const int rc = f.mt == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
+    if (rc != SA_OK || f.shares == 1) return rc;
+    return launch_join<HD>(c, F16, f.shares, P.part_o, P.part_lse, o, lse, st);
+}
+
+}  // namespace causal
+}  // namespace sa

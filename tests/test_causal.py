@@ -57,6 +57,10 @@ PACKED = [
     ([(5, 200), (64, 300), (1, 129)], 4, 2, 64, "fp16"),             # chunks over earlier keys
     ([(200, 40), (7, 0), (0, 9), (300, 299)], 2, 1, 128, "bf16"),    # more queries than keys: rows that see nothing
     ([(513, 513)], 3, 1, 64, "bf16"),
+    ([(1, 2001), (1, 1), (1, 64), (1, 0), (1, 65)], 16, 2, 128, "bf16"),       # single tokens
+    ([(3, 500), (7, 100), (4, 4), (2, 1), (0, 30)], 4, 1, 64, "fp16"),         # a few tokens: 28 rows
+    ([(2, 900), (1, 63)], 5, 5, 128, "fp16"),
+    ([(1, 300), (1, 128)], 24, 1, 64, "bf16"),
     ([(100, 100), (45, 70)], 2, 1, 80, "bf16"),                      # head dims of the general kernels
     ([(70, 70), (33, 97)], 2, 2, 256, "fp16"),
     ([(65, 65), (64, 100), (1, 7)], 4, 1, 64, "fp32"),
@@ -70,8 +74,8 @@ def test_packed_against_definition(case, algo):
     lens, H, Hkv, D, dtype = case
     (q, k, v, d_o), (cu_q, cu_k), seqs = make(lens, H, Hkv, D, dtype, seed=1)
     ref = causal_ref.reference(q, k, v, d_o, seqs, D ** -0.5)
-    compare(step(q, k, v, d_o, cu_q=cu_q, cu_k=cu_k), ref)
-    compare(step(q, k, v, d_o, cu_q=cu_q, cu_k=cu_k, max_q=max(n for n, _ in lens), max_k=max(m for _, m in lens)), ref)
+    for kw in ({}, dict(max_q=max(n for n, _ in lens), max_k=max(m for _, m in lens))):
+        compare(step(q, k, v, d_o, cu_q=cu_q, cu_k=cu_k, **kw), ref)
 
 
 @gpu
@@ -122,6 +126,25 @@ def test_later_keys_do_not_leak_forward(D, dtype, algo):
     ok[150 + 130:] = False
     assert torch.equal(before[ok], after[ok])
     assert not torch.isfinite(after[100:133, :, 5]).any() and torch.isnan(after[133:150]).all() and torch.isnan(after[280:]).all()
+
+
+@gpu
+@pytest.mark.parametrize("D,dtype", [(64, "bf16"), (128, "fp16")])
+def test_later_keys_do_not_leak_into_a_few_rows(D, dtype, algo):
+    lens = [(6, 150), (5, 131), (3, 8)]
+    (q, k, v, _), (cu_q, cu_k), _ = make(lens, 4, 1, D, dtype, seed=4)
+    call = lambda: sab.causal_attention(q, k, v, cu_q=cu_q, cu_k=cu_k, max_q=6, max_k=150)
+    before = call()
+    v[147, :, 5] = math.inf            # the last but two: queries 3 to 5 of the first sequence see it
+    k[150 + 129] = math.nan            # the last but one of the second
+    v[281 + 7] = -math.inf             # the last of the third
+    after = call()
+    ok = torch.ones_like(before, dtype=torch.bool)
+    ok[3:6, :, 5] = False
+    ok[9:11] = False
+    ok[13] = False
+    assert torch.equal(before[ok], after[ok])
+    assert not torch.isfinite(after[~ok]).any() and torch.isnan(after[9:11]).all()
 
 
 # B, N, M, H, Hkv, D, dtype, layout
@@ -410,6 +433,13 @@ def test_entries_validate():
     assert need >= 4 * 64 * 4 and bwd(params(), some, ctypes.c_void_p(256), need - 1) == 5
     assert bwd(params(), some, ctypes.c_void_p(128), need) == 5 and bwd(params(), some, nul, need) == 5
     assert lib.sa_causal_backward_workspace_size(params(D=0)) == 0
+    r = lambda b=0, **kw: lib.sa_causal_resolve(params(**kw), b)
+    assert r() == r(1) == r(1, Nq=1) == _abi.SA_ALGO_TCGEN05 and r(Nq=16) == _abi.SA_CAUSAL_FEW_ROWS and r(Nq=17) == _abi.SA_ALGO_TCGEN05
+    assert r(Nq=4, algo=_abi.SA_ALGO_TCGEN05) == _abi.SA_ALGO_TCGEN05 and r(sequences=9, max_q=1, max_k=5) == _abi.SA_CAUSAL_FEW_ROWS
+    for general in (dict(D=96), dict(dtype=_abi.SA_F32), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(algo=_abi.SA_ALGO_GENERAL),
+                    dict(k=_abi.Strides(64 * 512, 512, 132))):
+        assert r(**general) == r(1, **general) == _abi.SA_ALGO_GENERAL, general
+    assert r(D=96, algo=_abi.SA_ALGO_TCGEN05) == -4
     assert lib.sa_causal_resolve(params(D=257), 0) == -4 and lib.sa_causal_resolve(params(H=3), 1) == -2
 
 
