@@ -218,13 +218,15 @@ typedef struct {
     sa_strides d_o, dq, dk, dv;               /* backward tensors (ignored by sa_causal_forward) */
 } sa_causal_params;
 
-/* `status`: see sa_forward_status.  `workspace`: sa_causal_*_workspace_size() bytes, 256-byte aligned; NULL where that is 0. */
-int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, const void* v, void* o, float* lse,
-                      const int32_t* cu_q, const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status,
+/* `status`: see sa_forward_status.  `workspace`: sa_causal_*_workspace_size() bytes, 256-byte aligned; NULL where that is 0.
+ * `o_low` (NULL: not wanted) receives what rounding took from a 16-bit O, rounded to the same type, in O's strides: the backward
+ * forms sum_d dO O with it, whose error would else be a third of that of dQ and dK.  It holds rows of sequences only. */
+int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, const void* v, void* o, void* o_low,
+                      float* lse, const int32_t* cu_q, const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status,
                       void* stream);
-/* dq, dk and dv may be NULL.  Gradients are overwritten, without atomics, in a fixed order. */
+/* o_low, dq, dk and dv may be NULL.  Gradients are overwritten, without atomics, in a fixed order. */
 int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, const void* v, const void* o,
-                       const float* lse, const void* d_o, void* dq, void* dk, void* dv, const int32_t* cu_q,
+                       const void* o_low, const float* lse, const void* d_o, void* dq, void* dk, void* dv, const int32_t* cu_q,
                        const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status, void* stream);
 size_t sa_causal_forward_workspace_size(const sa_causal_params* p);
 size_t sa_causal_backward_workspace_size(const sa_causal_params* p);

@@ -101,9 +101,9 @@ def load():
     rp, cp = ctypes.POINTER(RotaryParams), ctypes.POINTER(CausalParams)
     lib.sa_rotary.argtypes = [rp] + [vp] * 5
     lib.sa_rotary.restype = ctypes.c_int
-    lib.sa_causal_forward.argtypes = [cp] + [vp] * 8 + [sz, vp, vp]
+    lib.sa_causal_forward.argtypes = [cp] + [vp] * 9 + [sz, vp, vp]
     lib.sa_causal_forward.restype = ctypes.c_int
-    lib.sa_causal_backward.argtypes = [cp] + [vp] * 12 + [sz, vp, vp]
+    lib.sa_causal_backward.argtypes = [cp] + [vp] * 13 + [sz, vp, vp]
     lib.sa_causal_backward.restype = ctypes.c_int
     lib.sa_causal_forward_workspace_size.argtypes = [cp]
     lib.sa_causal_forward_workspace_size.restype = sz

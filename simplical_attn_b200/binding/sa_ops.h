@@ -267,7 +267,9 @@ struct Scratch {
 };
 const int32_t* ints(const Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; }
 
-std::pair<Tensor, Tensor> causal_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu_q, const Tensor& cu_k, const CausalConfig& c) {
+// O, LSE, and with `low` what rounding took from a 16-bit O (else, and for fp32, undefined).
+std::array<Tensor, 3> causal_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& cu_q, const Tensor& cu_k, const CausalConfig& c,
+                                     bool low) {
     check_causal(q_, k_, v_, cu_q, cu_k);
     const c10::cuda::CUDAGuard guard(q_.device());
     const Tensor q = unit_inner(q_), k = unit_inner(k_), v = unit_inner(v_);
@@ -279,18 +281,20 @@ std::pair<Tensor, Tensor> causal_forward(const Tensor& q_, const Tensor& k_, con
     if (q.numel() == 0 || k.numel() == 0) {                // no query, or none that sees a key
         o.zero_();
         lse.fill_(-std::numeric_limits<float>::infinity());
-        return {std::move(o), std::move(lse)};
+        return {std::move(o), std::move(lse), Tensor()};
     }
+    Tensor o_low;
+    if (low && q.scalar_type() != at::kFloat) o_low = at::empty_like(o);
     const sa_causal_params p = causal_params(q, k, v, o, cu_q, c);
     const Scratch ws(sa_causal_forward_workspace_size(&p), q);
-    const int rc = sa_causal_forward(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), (float*)lse.data_ptr(), ints(cu_q), ints(cu_k), ws.ptr,
-                                     ws.bytes, status_word(device, kCausalForward), at::cuda::getCurrentCUDAStream(device).stream());
+    const int rc = sa_causal_forward(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), o_low.defined() ? o_low.data_ptr() : nullptr,
+                                     (float*)lse.data_ptr(), ints(cu_q), ints(cu_k), ws.ptr, ws.bytes, status_word(device, kCausalForward), at::cuda::getCurrentCUDAStream(device).stream());
     if (rc != SA_OK) raise_status("sa_causal_forward", rc);
-    return {std::move(o), std::move(lse)};
+    return {std::move(o), std::move(lse), std::move(o_low)};
 }
 
-std::array<Tensor, 3> causal_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& o_, const Tensor& lse, const Tensor& d_o_,
-                                      const Tensor& cu_q, const Tensor& cu_k, const CausalConfig& c, const std::array<bool, 3>& need) {
+std::array<Tensor, 3> causal_backward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& o_, const Tensor& o_low, const Tensor& lse,
+                                      const Tensor& d_o_, const Tensor& cu_q, const Tensor& cu_k, const CausalConfig& c, const std::array<bool, 3>& need) {
     check_causal(q_, k_, v_, cu_q, cu_k);
     TORCH_CHECK_TYPE(d_o_.scalar_type() == q_.scalar_type() && d_o_.device() == q_.device() && o_.scalar_type() == q_.scalar_type() && o_.device() == q_.device(),
                      "o and its gradient must match q's dtype and device");
@@ -300,6 +304,9 @@ std::array<Tensor, 3> causal_backward(const Tensor& q_, const Tensor& k_, const 
                       "lse must be the forward's");
     const c10::cuda::CUDAGuard guard(q_.device());
     const Tensor q = unit_inner(q_), k = unit_inner(k_), v = unit_inner(v_), o = unit_inner(o_), d_o = unit_inner(d_o_);
+    TORCH_CHECK_VALUE(!o_low.defined() || (o_low.sizes() == o.sizes() && o_low.strides() == o.strides() && o_low.scalar_type() == o.scalar_type() &&
+                                           o_low.device() == o.device()),
+                      "o_low must be the forward's");
     const int device = q.device().index();
     poll_device(device);
     const Tensor* const in[3] = {&q, &k, &v};
@@ -315,15 +322,15 @@ std::array<Tensor, 3> causal_backward(const Tensor& q_, const Tensor& k_, const 
     p.d_o = row_strides(d_o);
     p.dq = row_strides(g[0]); p.dk = row_strides(g[1]); p.dv = row_strides(g[2]);
     const Scratch ws(sa_causal_backward_workspace_size(&p), q);
-    const int rc = sa_causal_backward(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), (const float*)lse.data_ptr(), d_o.data_ptr(), gp[0], gp[1],
-                                      gp[2], ints(cu_q), ints(cu_k), ws.ptr, ws.bytes, status_word(device, kCausalBackward),
+    const int rc = sa_causal_backward(&p, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), o_low.defined() ? o_low.data_ptr() : nullptr,
+                                      (const float*)lse.data_ptr(), d_o.data_ptr(), gp[0], gp[1], gp[2], ints(cu_q), ints(cu_k), ws.ptr, ws.bytes, status_word(device, kCausalBackward),
                                       at::cuda::getCurrentCUDAStream(device).stream());
     if (rc != SA_OK) raise_status("sa_causal_backward", rc);
     return g;
 }
 
 struct CausalBackward : public torch::autograd::Node {
-    torch::autograd::SavedVariable q, k, v, o, lse, cu_q, cu_k;
+    torch::autograd::SavedVariable q, k, v, o, o_low, lse, cu_q, cu_k;
     CausalConfig cfg;
 
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
@@ -335,17 +342,17 @@ struct CausalBackward : public torch::autograd::Node {
         for (int i = 0; i < 3; ++i) any |= need[i] = task_should_compute_output(i);
         if (!any) return out;
         const auto self = getptr();
-        const Tensor q_ = q.unpack(), k_ = k.unpack(), v_ = v.unpack(), o_ = o.unpack(self), lse_ = lse.unpack(), cq = cu_q.unpack(), ck = cu_k.unpack();
+        const Tensor q_ = q.unpack(), k_ = k.unpack(), v_ = v.unpack(), o_ = o.unpack(self), low_ = o_low.unpack(), lse_ = lse.unpack(), cq = cu_q.unpack(), ck = cu_k.unpack();
         {
             at::AutoDispatchBelowADInplaceOrView below;
-            std::array<Tensor, 3> g = causal_backward(q_, k_, v_, o_, lse_, grads[0], cq, ck, cfg, need);
+            std::array<Tensor, 3> g = causal_backward(q_, k_, v_, o_, low_, lse_, grads[0], cq, ck, cfg, need);
             for (int i = 0; i < 3; ++i) out[i] = std::move(g[i]);
         }
         return at::GradMode::is_enabled() ? no_second_derivative(std::move(out), "causal_attention") : out;
     }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
-        for (auto* x : {&q, &k, &v, &o, &lse, &cu_q, &cu_k}) x->reset_data();
+        for (auto* x : {&q, &k, &v, &o, &o_low, &lse, &cu_q, &cu_k}) x->reset_data();
     }
     std::string name() const override { return "CausalAttentionBackward"; }
 };
@@ -362,17 +369,18 @@ std::pair<Tensor, Tensor> causal_attention(const Tensor& q, const Tensor& k, con
         node->cu_q = torch::autograd::SavedVariable(cu_q, false);
         node->cu_k = torch::autograd::SavedVariable(cu_k, false);
     }
-    std::pair<Tensor, Tensor> r;
+    std::array<Tensor, 3> r;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        r = causal_forward(q, k, v, cu_q, cu_k, c);
+        r = causal_forward(q, k, v, cu_q, cu_k, c, node != nullptr);
     }
     if (node) {
-        torch::autograd::set_history(r.first, node);
-        node->o = torch::autograd::SavedVariable(r.first, true);
-        node->lse = torch::autograd::SavedVariable(r.second, false);
+        torch::autograd::set_history(r[0], node);
+        node->o = torch::autograd::SavedVariable(r[0], true);
+        node->lse = torch::autograd::SavedVariable(r[1], false);
+        node->o_low = torch::autograd::SavedVariable(r[2], false);
     }
-    return r;
+    return {std::move(r[0]), std::move(r[1])};
 }
 
 // ---------------------------------------------------------------------------------------- Python entry points
@@ -446,41 +454,42 @@ PyObject* py_causal(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// the same without a history
+// the same and whether O's low part is wanted; without a history
 PyObject* py_causal_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    expect(n, 9);
+    expect(n, 10);
     if (!exact(a, 3)) Py_RETURN_NONE;
     const Tensor &q = tensor_arg(a[0], "q"), &k = tensor_arg(a[1], "k"), &v = tensor_arg(a[2], "v");
     const Tensor cu_q = optional_tensor(a[3], "cu_q"), cu_k = optional_tensor(a[4], "cu_k");
     const CausalConfig c = causal_config(a + 5);
-    std::pair<Tensor, Tensor> r;
+    const bool low = int_arg(a[9]) != 0;
+    std::array<Tensor, 3> r;
     {
         pybind11::gil_scoped_release no_gil;
         at::AutoDispatchBelowADInplaceOrView below;
-        r = causal_forward(q, k, v, cu_q, cu_k, c);
+        r = causal_forward(q, k, v, cu_q, cu_k, c, low);
     }
-    return wrap_tuple({std::move(r.first), std::move(r.second)});
+    return wrap_tuple({std::move(r[0]), std::move(r[1]), std::move(r[2])});
     END_HANDLE_TH_ERRORS
 }
 
-// q, k, v, o, lse, d_o, cu_q or None, cu_k or None, scale, max_q, max_k, algo, need (bit i: gradient i)
+// q, k, v, o, lse, d_o, o_low or None, cu_q or None, cu_k or None, scale, max_q, max_k, algo, need (bit i: gradient i)
 PyObject* py_causal_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    expect(n, 13);
+    expect(n, 14);
     if (!exact(a, 6)) Py_RETURN_NONE;
     static const char* const names[6] = {"q", "k", "v", "o", "lse", "d_o"};
     const Tensor* t[6];
     for (int i = 0; i < 6; ++i) t[i] = &tensor_arg(a[i], names[i]);
-    const Tensor cu_q = optional_tensor(a[6], "cu_q"), cu_k = optional_tensor(a[7], "cu_k");
-    const CausalConfig c = causal_config(a + 8);
-    const int64_t bits = int_arg(a[12]);
+    const Tensor o_low = optional_tensor(a[6], "o_low"), cu_q = optional_tensor(a[7], "cu_q"), cu_k = optional_tensor(a[8], "cu_k");
+    const CausalConfig c = causal_config(a + 9);
+    const int64_t bits = int_arg(a[13]);
     const std::array<bool, 3> need{(bits & 1) != 0, (bits & 2) != 0, (bits & 4) != 0};
     std::array<Tensor, 3> g;
     {
         pybind11::gil_scoped_release no_gil;
         at::AutoDispatchBelowADInplaceOrView below;
-        g = causal_backward(*t[0], *t[1], *t[2], *t[3], *t[4], *t[5], cu_q, cu_k, c, need);
+        g = causal_backward(*t[0], *t[1], *t[2], *t[3], o_low, *t[4], *t[5], cu_q, cu_k, c, need);
     }
     return wrap_tuple({std::move(g[0]), std::move(g[1]), std::move(g[2])});
     END_HANDLE_TH_ERRORS

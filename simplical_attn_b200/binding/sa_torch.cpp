@@ -424,7 +424,7 @@ PyMethodDef kMethods[] = {
     {"backward", (PyCFunction)(void*)py_backward, METH_FASTCALL, "(dq, dk1, dk2, dv1, dv2); None for tensor subclasses"},
     {"rotary", (PyCFunction)(void*)py_rotary, METH_FASTCALL, "the rotated tensors with their autograd history; None if the call is not plain"},
     {"causal_attention", (PyCFunction)(void*)py_causal, METH_FASTCALL, "(O, LSE), O with its autograd history; None if the call is not plain"},
-    {"causal_forward", (PyCFunction)(void*)py_causal_forward, METH_FASTCALL, "(O, LSE); None for tensor subclasses"},
+    {"causal_forward", (PyCFunction)(void*)py_causal_forward, METH_FASTCALL, "(O, LSE, low part of O or None); None for tensor subclasses"},
     {"causal_backward", (PyCFunction)(void*)py_causal_backward, METH_FASTCALL, "(dq, dk, dv); None for tensor subclasses"},
     {"poll", py_poll, METH_O, "raises if an earlier call on the device left a status"},
     {"status_word", (PyCFunction)(void*)py_status_word, METH_FASTCALL, "address of the word that calls of a device and direction report to"},

@@ -68,19 +68,20 @@ def _with_status(size, device):
     return _host._workspace(256 + size, device)
 
 
-def causal_attention_fwd(q, k, v, scale, cu_q=None, cu_k=None, max_q=0, max_k=0, algo=None):
-    """Forward launch: (O, LSE), LSE fp32 [B, H, N] (packed: [H, rows])."""
+def causal_attention_fwd(q, k, v, scale, cu_q=None, cu_k=None, max_q=0, max_k=0, algo=None, low=False):
+    """Forward launch: (O, LSE), LSE fp32 [B, H, N] (packed: [H, rows]).  With `low` also what rounding took from a 16-bit O
+    (None for fp32), which the backward forms sum dO O with: without it dQ and dK are about 5 % less exact."""
     algo = algo or _host.default_algo
     cu_k = cu_q if cu_k is None else cu_k
     if _host._status_watch.active:
         _host._status_watch.poll(q.device)
     native = _native()
     if native is not None:
-        out = native.causal_forward(q, k, v, cu_q, cu_k, scale, max_q, max_k, _ALGOS[algo])
+        out = native.causal_forward(q, k, v, cu_q, cu_k, scale, max_q, max_k, _ALGOS[algo], low)
         if out is not None:
             if _host.debug_device_status:
                 _host._status_watch.flush(q.device)
-            return out
+            return out if low else out[:2]
     _check(q, k, v, cu_q, cu_k)
     lib = _abi.load()
     q, k, v = (_unit_inner(t) for t in (q, k, v))
@@ -88,18 +89,19 @@ def causal_attention_fwd(q, k, v, scale, cu_q=None, cu_k=None, max_q=0, max_k=0,
         o = torch.empty_like(q)
         lse = torch.empty((*q.shape[:-3], q.shape[-2], q.shape[-3]), device=q.device, dtype=torch.float32)
         if q.numel() == 0 or k.numel() == 0:
-            return o.zero_(), lse.fill_(-math.inf)
+            return (o.zero_(), lse.fill_(-math.inf)) + ((None,) if low else ())
+        o_low = torch.empty_like(o) if low and q.dtype != torch.float32 else None
         p = _params(q, k, v, o, cu_q, scale, max_q, max_k, algo)
         ws = _with_status(lib.sa_causal_forward_workspace_size(ctypes.byref(p)), q.device)
         sh = torch.cuda.current_stream().cuda_stream
-        rc = lib.sa_causal_forward(ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(cu_q), _ptr(cu_k),
+        rc = lib.sa_causal_forward(ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(o_low), _ptr(lse), _ptr(cu_q), _ptr(cu_k),
                                    ws.data_ptr() + 256, ws.numel() - 256, _ptr(ws), ctypes.c_void_p(sh))
         _abi.check("sa_causal_forward", rc)
         _host._status(lib, ws, "sa_causal_forward", sh)
-    return o, lse
+    return (o, lse, o_low) if low else (o, lse)
 
 
-def causal_attention_bwd(q, k, v, o, lse, d_o, scale, cu_q=None, cu_k=None, max_q=0, max_k=0, need=(True, True, True), algo=None):
+def causal_attention_bwd(q, k, v, o, lse, d_o, scale, cu_q=None, cu_k=None, max_q=0, max_k=0, need=(True, True, True), algo=None, o_low=None):
     """Backward launches: (dq, dk, dv), `None` where `need[i]` is false."""
     algo = algo or _host.default_algo
     cu_k = cu_q if cu_k is None else cu_k
@@ -108,7 +110,7 @@ def causal_attention_bwd(q, k, v, o, lse, d_o, scale, cu_q=None, cu_k=None, max_
     native = _native()
     if native is not None:
         bits = sum(1 << i for i, n in enumerate(need) if n)
-        grads = native.causal_backward(q, k, v, o, lse, d_o, cu_q, cu_k, scale, max_q, max_k, _ALGOS[algo], bits)
+        grads = native.causal_backward(q, k, v, o, lse, d_o, o_low, cu_q, cu_k, scale, max_q, max_k, _ALGOS[algo], bits)
         if grads is not None:
             if _host.debug_device_status:
                 _host._status_watch.flush(q.device)
@@ -121,6 +123,8 @@ def causal_attention_bwd(q, k, v, o, lse, d_o, scale, cu_q=None, cu_k=None, max_
             raise ValueError("o and its gradient must have q's shape")
     if lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous() or lse.shape != (*q.shape[:-3], q.shape[-2], q.shape[-3]):
         raise ValueError("lse must be the forward's")
+    if o_low is not None and (o_low.shape != o.shape or o_low.stride() != o.stride() or o_low.dtype != o.dtype or o_low.device != o.device):
+        raise ValueError("o_low must be the forward's")
     lib = _abi.load()
     q, k, v, o, d_o = (_unit_inner(t) for t in (q, k, v, o, d_o))
     with torch.cuda.device(q.device):
@@ -132,7 +136,7 @@ def causal_attention_bwd(q, k, v, o, lse, d_o, scale, cu_q=None, cu_k=None, max_
         p.dq, p.dk, p.dv = (_abi.Strides(0, 0, 0) if g is None else _row_strides(g) for g in grads)
         ws = _with_status(lib.sa_causal_backward_workspace_size(ctypes.byref(p)), q.device)
         sh = torch.cuda.current_stream().cuda_stream
-        rc = lib.sa_causal_backward(ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(lse), _ptr(d_o), *[_ptr(g) for g in grads],
+        rc = lib.sa_causal_backward(ctypes.byref(p), _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(o_low), _ptr(lse), _ptr(d_o), *[_ptr(g) for g in grads],
                                     _ptr(cu_q), _ptr(cu_k), ws.data_ptr() + 256, ws.numel() - 256, _ptr(ws), ctypes.c_void_p(sh))
         _abi.check("sa_causal_backward", rc)
         _host._status(lib, ws, "sa_causal_backward", sh)
@@ -144,8 +148,8 @@ class CausalAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, scale, max_q, max_k):
-        o, lse = causal_attention_fwd(q, k, v, scale, cu_q, cu_k, max_q, max_k)
-        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k)
+        o, lse, o_low = causal_attention_fwd(q, k, v, scale, cu_q, cu_k, max_q, max_k, None, True)
+        ctx.save_for_backward(q, k, v, o, lse, o_low, cu_q, cu_k)
         ctx.cfg = (scale, max_q, max_k)
         ctx.mark_non_differentiable(lse)
         return o, lse
@@ -153,10 +157,10 @@ class CausalAttentionFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output, _):
-        q, k, v, o, lse, cu_q, cu_k = ctx.saved_tensors
+        q, k, v, o, lse, o_low, cu_q, cu_k = ctx.saved_tensors
         scale, max_q, max_k = ctx.cfg
         need = tuple(bool(n) for n in ctx.needs_input_grad[:3])
-        return causal_attention_bwd(q, k, v, o, lse, grad_output, scale, cu_q, cu_k, max_q, max_k, need) + (None,) * 5
+        return causal_attention_bwd(q, k, v, o, lse, grad_output, scale, cu_q, cu_k, max_q, max_k, need, o_low=o_low) + (None,) * 5
 
 
 def causal_attention(q, k, v, scale: Optional[float] = None, *, cu_q: Optional[torch.Tensor] = None,

@@ -62,7 +62,7 @@ int resolve(const sa_causal_params* p, bool backward) {
     if (p->algo == SA_ALGO_TCGEN05) return ok ? SA_ALGO_TCGEN05 : -SA_ERR_UNSUPPORTED;
     if (!ok) return SA_ALGO_GENERAL;
     const CParams c = make_params(p, nullptr, nullptr);
-    return !backward && (int64_t)c.max_q * c.G <= kFewRowsMost ? SA_CAUSAL_FEW_ROWS : SA_ALGO_TCGEN05;
+    return !backward && (int64_t)c.max_q * c.G <= kFewRowsMost ? (int)SA_CAUSAL_FEW_ROWS : (int)SA_ALGO_TCGEN05;
 }
 
 // (a plan only asks whether there are starts)
@@ -113,8 +113,8 @@ int sa_causal_resolve(const sa_causal_params* p, int backward) {
     return rc != SA_OK ? -rc : resolve(p, backward != 0);
 }
 
-int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* cu_q,
-                      const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status, void* stream) {
+int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, const void* v, void* o, void* o_low, float* lse,
+                      const int32_t* cu_q, const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status, void* stream) {
     using namespace sa::causal;
     int rc = validate(p);
     if (rc != SA_OK) return rc;
@@ -127,21 +127,21 @@ int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, c
     if (algo != SA_ALGO_GENERAL) {
         if (sa::host::cc_major() != 10) return SA_ERR_NOT_SM100;
         rc = SA_ERR_BAD_STRIDE;
-        if (sa::host::aligned16(q) && sa::host::aligned16(k) && sa::host::aligned16(v) && sa::host::aligned16(o))
+        if (sa::host::aligned16(q) && sa::host::aligned16(k) && sa::host::aligned16(v) && sa::host::aligned16(o) && sa::host::aligned16(o_low))
             rc = dispatch_tc(p, [&](auto d, auto f16) {
                 if (algo == SA_CAUSAL_FEW_ROWS)
-                    return launch_few<decltype(d)::value, decltype(f16)::value>(c, q, k, v, o, lse, static_cast<uint8_t*>(workspace), st);
-                return launch_fwd_tc<decltype(d)::value, decltype(f16)::value>(c, q, k, v, o, lse, static_cast<uint8_t*>(workspace),
+                    return launch_few<decltype(d)::value, decltype(f16)::value>(c, q, k, v, o, o_low, lse, static_cast<uint8_t*>(workspace), st);
+                return launch_fwd_tc<decltype(d)::value, decltype(f16)::value>(c, q, k, v, o, o_low, lse, static_cast<uint8_t*>(workspace),
                                                                              static_cast<sa::DeviceStatus*>(status), st);
             });
         // (BAD_STRIDE: nothing has been launched)
         if (rc != SA_ERR_BAD_STRIDE || p->algo == SA_ALGO_TCGEN05) return rc;
     }
-    return dispatch_general(p->dtype, p->D, [&](auto t, auto d) { return launch_general_fwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, lse, st); });
+    return dispatch_general(p->dtype, p->D, [&](auto t, auto d) { return launch_general_fwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, o_low, lse, st); });
 }
 
-int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o,
-                       void* dq, void* dk, void* dv, const int32_t* cu_q, const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status,
+int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, const void* v, const void* o, const void* o_low, const float* lse,
+                       const void* d_o, void* dq, void* dk, void* dv, const int32_t* cu_q, const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status,
                        void* stream) {
     using namespace sa::causal;
     int rc = validate(p);
@@ -158,16 +158,16 @@ int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, 
         if (sa::host::cc_major() != 10) return SA_ERR_NOT_SM100;
         rc = SA_ERR_BAD_STRIDE;
         bool aligned = true;
-        for (const void* x : {q, k, v, o, d_o, (const void*)dq, (const void*)dk, (const void*)dv}) aligned = aligned && sa::host::aligned16(x);
+        for (const void* x : {q, k, v, o, o_low, d_o, (const void*)dq, (const void*)dk, (const void*)dv}) aligned = aligned && sa::host::aligned16(x);
         if (aligned)
             rc = dispatch_tc(p, [&](auto d, auto f16) {
-                return launch_bwd_tc<decltype(d)::value, decltype(f16)::value>(c, q, k, v, o, lse, d_o, dq, dk, dv, static_cast<uint8_t*>(workspace),
+                return launch_bwd_tc<decltype(d)::value, decltype(f16)::value>(c, q, k, v, o, o_low, lse, d_o, dq, dk, dv, static_cast<uint8_t*>(workspace),
                                                                              static_cast<sa::DeviceStatus*>(status), st);
             });
         if (rc != SA_ERR_BAD_STRIDE || p->algo == SA_ALGO_TCGEN05) return rc;
     }
     return dispatch_general(p->dtype, p->D, [&](auto t, auto d) {
-        return launch_general_bwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, lse, d_o, dq, dk, dv, delta, st);
+        return launch_general_bwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, o_low, lse, d_o, dq, dk, dv, delta, st);
     });
 }
 

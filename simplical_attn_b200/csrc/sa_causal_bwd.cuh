@@ -39,8 +39,8 @@ struct BwdParams {
 
 // Delta, eight elements a lane.
 template <int HD, bool F16>
-__global__ void __launch_bounds__(256) causal_delta16_kernel(const CParams p, const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ d_o,
-                                                            float* __restrict__ delta) {
+__global__ void __launch_bounds__(256) causal_delta16_kernel(const CParams p, const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o_low,
+                                                            const __nv_bfloat16* __restrict__ d_o, float* __restrict__ delta) {
     using E = ptx::El<F16>;
     constexpr int kLanes = HD / 8;
     const int lane = threadIdx.x % kLanes;
@@ -52,13 +52,14 @@ __global__ void __launch_bounds__(256) causal_delta16_kernel(const CParams p, co
         h = (int)(w % p.H);
         i = (int)(w / p.H % p.Nq);
         b = (int)(w / p.H / p.Nq);
-        const uint4 x = *reinterpret_cast<const uint4*>(o + b * p.o.b + i * p.o.n + h * p.o.h + 8 * lane);
+        const int64_t at = b * p.o.b + i * p.o.n + h * p.o.h + 8 * lane;
+        const uint4 x = *reinterpret_cast<const uint4*>(o + at), z = o_low ? *reinterpret_cast<const uint4*>(o_low + at) : make_uint4(0, 0, 0, 0);
         const uint4 y = *reinterpret_cast<const uint4*>(d_o + b * p.d_o.b + i * p.d_o.n + h * p.d_o.h + 8 * lane);
-        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w}, zw[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            sum = fmaf(E::lo(xw[e]), E::lo(yw[e]), sum);
-            sum = fmaf(E::hi(xw[e]), E::hi(yw[e]), sum);
+            sum = fmaf(E::lo(xw[e]) + E::lo(zw[e]), E::lo(yw[e]), sum);
+            sum = fmaf(E::hi(xw[e]) + E::hi(zw[e]), E::hi(yw[e]), sum);
         }
     }
 #pragma unroll
@@ -921,8 +922,8 @@ inline BwdPlan plan_bwd(const CParams& c) {
 }
 
 template <int HD, bool F16>
-int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, void* dq, void* dk,
-                  void* dv, uint8_t* ws, DeviceStatus* status, cudaStream_t st) {
+int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v, const void* o, const void* o_low, const float* lse, const void* d_o,
+                  void* dq, void* dk, void* dv, uint8_t* ws, DeviceStatus* status, cudaStream_t st) {
     const BwdPlan f = plan_bwd(c);
     if (f.items_q * c.H * f.splits_q > 0x3fffffff || f.items_k * c.Hkv * f.splits_k > 0x3fffffff) return SA_ERR_UNSUPPORTED;
     CUtensorMap mq, mk, mv, mo;
@@ -935,7 +936,8 @@ int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v,
     float* delta = reinterpret_cast<float*>(ws + f.delta);
     const int64_t rows = (int64_t)c.B * c.Nq * c.H;
     constexpr int kPerBlock = 256 / (HD / 8);
-    causal_delta16_kernel<HD, F16><<<(unsigned)((rows + kPerBlock - 1) / kPerBlock), 256, 0, st>>>(c, (const __nv_bfloat16*)o, (const __nv_bfloat16*)d_o, delta);
+    causal_delta16_kernel<HD, F16><<<(unsigned)((rows + kPerBlock - 1) / kPerBlock), 256, 0, st>>>(c, (const __nv_bfloat16*)o, (const __nv_bfloat16*)o_low,
+                                                                                                     (const __nv_bfloat16*)d_o, delta);
     host::count_launches(1);
     BwdParams P{};
     P.c = c;

@@ -21,6 +21,7 @@ constexpr int kFewRowsMost = 32;          // rows (queries times heads of a grou
 struct FewParams {
     CParams c;
     int shares, row_blocks;               // of a sequence's keys, and of its rows
+    int steps;                            // steps of a share, at least
     float* part_o;                        // shares > 1: as in FwdParams
     float* part_lse;
 };
@@ -70,7 +71,7 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
 template <int HD, bool F16, int MT>
 __global__ void __launch_bounds__(kFewThreads, MT == 1 ? 2 : 2)
 causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ k,
-                  const __nv_bfloat16* __restrict__ v, __nv_bfloat16* __restrict__ o, float* __restrict__ lse) {
+                  const __nv_bfloat16* __restrict__ v, __nv_bfloat16* __restrict__ o, __nv_bfloat16* __restrict__ o_low, float* __restrict__ lse) {
     using L = FewLayout<HD, MT>;
     using E = ptx::El<F16>;
     constexpr int kChunks = HD / 8;               // 16-byte chunks of a row
@@ -89,9 +90,9 @@ causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __re
     const Seq s = seq_of(p, x / p.Hkv);
     const int R = s.nq * p.G;
     const int64_t rows_all = (int64_t)p.B * p.H * p.Nq;
-    // whole steps of keys per share, as many as the sequence needs
-    const int steps_all = (s.nk + kFewKeys - 1) / kFewKeys, per = (steps_all + P.shares - 1) / P.shares;
-    const int c0 = min(share * per * kFewKeys, s.nk), c1 = min(c0 + per * kFewKeys, s.nk);
+    // equal shares for sequences of all lengths: short ones have fewer (and one longer than max_k said has longer ones)
+    const int steps_all = (s.nk + kFewKeys - 1) / kFewKeys, per = max(P.steps, (steps_all + P.shares - 1) / P.shares);
+    const int c0 = min(min(share * per, steps_all) * kFewKeys, s.nk), c1 = min(c0 + per * kFewKeys, s.nk);
     const int steps = (c1 - c0 + kFewKeys - 1) / kFewKeys;
 
     const uint32_t q_st = ptx::smem_u32(smem), w_st = q_st + L::kQ + L::kStats + warp * L::kWarp;
@@ -325,8 +326,12 @@ causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __re
                 if (!none) *reinterpret_cast<float4*>(P.part_o + (share * rows_all + at) * HD + d) = make_float4(t.x * inv, t.y * inv, t.z * inv, t.w * inv);
                 if (d == 0) P.part_lse[share * rows_all + at] = ll;
             } else {
-                *reinterpret_cast<uint2*>(o + s.b * p.o.b + (int64_t)(s.q0 + i) * p.o.n + h * p.o.h + d) =
-                    make_uint2(E::pack(t.x * inv, t.y * inv), E::pack(t.z * inv, t.w * inv));
+                const int64_t dst = s.b * p.o.b + (int64_t)(s.q0 + i) * p.o.n + h * p.o.h + d;
+                uint2 y, low;
+                pack_split<F16>(t.x * inv, t.y * inv, y.x, low.x);
+                pack_split<F16>(t.z * inv, t.w * inv, y.y, low.y);
+                *reinterpret_cast<uint2*>(o + dst) = y;
+                if (o_low) *reinterpret_cast<uint2*>(o_low + dst) = low;
                 if (d == 0) lse[at] = ll;
             }
         }
@@ -339,23 +344,36 @@ causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __re
 }
 
 struct FewPlan {
-    int mt, shares, row_blocks;
+    int mt, shares, steps, row_blocks;
     size_t part_o, part_lse, bytes;
 };
+// Shares of the keys, by an estimate of the time: a round of resident blocks (two to a multiprocessor) costs 1.5 us before its
+// first and after its last step; a step takes 1 us, or what its bytes take of the bandwidth where all of them run; joining
+// takes 3 us and 0.05 for every share.
 inline FewPlan plan_few(const CParams& c) {
     FewPlan f{};
     const int rows = (int)((int64_t)c.max_q * c.G < kFewRowsMost ? c.max_q * c.G : kFewRowsMost);
     f.mt = rows > 16 ? 2 : 1;
     f.row_blocks = ceil_div(rows, 16 * f.mt);
-    // Shares of at least four steps, enough for three rounds of blocks over the multiprocessors (two at a time each): packed
-    // sequences are shorter than the longest, so theirs are cut by the mean.
-    const int64_t blocks = (int64_t)c.S * c.Hkv * f.row_blocks, want = 6 * host::sm_count();
-    const int64_t mean = c.cu_q != nullptr && c.Nk / c.S < c.max_k ? (c.Nk / c.S > 0 ? c.Nk / c.S : 1) : c.max_k;
-    int64_t shares = (want * c.max_k / mean + blocks - 1) / blocks;
-    const int64_t most = ceil_div(c.max_k, 4 * kFewKeys);
-    if (shares > most) shares = most;
-    if (shares > 256) shares = 256;
-    f.shares = shares < 1 ? 1 : (int)shares;
+    const bool packed = c.cu_q != nullptr;
+    const int longest = ceil_div(c.max_k, kFewKeys);
+    const double heads = (double)c.Hkv * f.row_blocks, slots = 2.0 * host::sm_count();
+    const double total = packed ? (double)c.Nk / kFewKeys + 0.5 * c.S : (double)longest * c.S;      // steps of a head
+    double best = 1e30;
+    for (int n = 1; n <= 128 && n <= longest; ++n) {
+        const int per = ceil_div(longest, n);
+        if (n > 1 && per == ceil_div(longest, n - 1)) continue;
+        const double blocks = heads * (packed ? (total / per < c.S ? c.S : total / per + 0.5 * c.S) : (double)ceil_div(longest, per) * c.S);
+        double rounds = blocks / slots;
+        rounds = rounds <= 1 ? 1 : rounds < 4 ? (double)(int)(rounds + 0.999) : rounds + 0.5;
+        const double running = blocks < slots ? blocks : slots, bound = kFewKeys * c.D * 4.0 * running / 6.2e6;
+        const double us = rounds * (1.5 + per * (bound > 1.0 ? bound : 1.0)) + (n > 1 ? 3.0 + 0.05 * n : 0.0);
+        if (us < best) {
+            best = us;
+            f.shares = ceil_div(longest, per);
+            f.steps = per;
+        }
+    }
     const size_t all = (size_t)c.B * c.H * c.Nq;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };
@@ -366,13 +384,14 @@ inline FewPlan plan_few(const CParams& c) {
 }
 
 template <int HD, bool F16>
-int launch_few(const CParams& c, const void* q, const void* k, const void* v, void* o, float* lse, uint8_t* ws, cudaStream_t st) {
+int launch_few(const CParams& c, const void* q, const void* k, const void* v, void* o, void* o_low, float* lse, uint8_t* ws, cudaStream_t st) {
     const FewPlan f = plan_few(c);
     const int64_t grid = (int64_t)c.S * c.Hkv * f.row_blocks * f.shares;
     if (grid > 0x7fffffff) return SA_ERR_UNSUPPORTED;
     FewParams P{};
     P.c = c;
     P.shares = f.shares;
+    P.steps = f.steps;
     P.row_blocks = f.row_blocks;
     P.part_o = reinterpret_cast<float*>(ws + f.part_o);
     P.part_lse = reinterpret_cast<float*>(ws + f.part_lse);
@@ -381,13 +400,13 @@ int launch_few(const CParams& c, const void* q, const void* k, const void* v, vo
         auto kern = causal_few_kernel<HD, F16, MT>;
         if (!allow_dynamic_smem((const void*)kern, FewLayout<HD, MT>::kBytes)) return SA_ERR_LAUNCH;
         kern<<<(unsigned)grid, kFewThreads, FewLayout<HD, MT>::kBytes, st>>>(P, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v,
-                                                                             (__nv_bfloat16*)o, lse);
+                                                                             (__nv_bfloat16*)o, (__nv_bfloat16*)o_low, lse);
         host::count_launches(1);
         return cudaGetLastError() == cudaSuccess ? SA_OK : SA_ERR_LAUNCH;
     };
     const int rc = f.mt == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
     if (rc != SA_OK || f.shares == 1) return rc;
-    return launch_join<HD>(c, F16, f.shares, P.part_o, P.part_lse, o, lse, st);
+    return launch_join<HD>(c, F16, f.shares, P.part_o, P.part_lse, o, o_low, lse, st);
 }
 
 }  // namespace causal

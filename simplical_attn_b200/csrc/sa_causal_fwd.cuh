@@ -109,10 +109,18 @@ struct Ring {
     }
 };
 
+// Two values as packed 16-bit ones, and what that rounding took from them.
+template <bool F16>
+__device__ __forceinline__ void pack_split(float a, float b, uint32_t& w, uint32_t& low) {
+    using E = ptx::El<F16>;
+    w = E::pack(a, b);
+    low = E::pack(a - E::lo(w), b - E::hi(w));
+}
+
 template <int HD, bool F16>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                     const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ o, float* __restrict__ lse) {
+                     const __grid_constant__ CUtensorMap map_v, __nv_bfloat16* __restrict__ o, __nv_bfloat16* __restrict__ o_low, float* __restrict__ lse) {
     using L = FwdLayout<HD>;
     using namespace ptx;
     using E = El<F16>;
@@ -457,7 +465,7 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
             }
             const float inv = none ? 0.f : 1.f / l;
             const bool noted = *bad_unit == (int)units + 1;
-            __nv_bfloat16* const out = o + u.s.b * p.o.b + (int64_t)(u.s.q0 + i) * p.o.n + u.h * p.o.h;
+            const int64_t out_at = u.s.b * p.o.b + (int64_t)(u.s.q0 + i) * p.o.n + u.h * p.o.h;
             float* const part = P.splits > 1 ? P.part_o + ((int64_t)u.split * rows + at) * HD : nullptr;
 #pragma unroll 1
             for (int c0 = 0; c0 < HD; c0 += 32) {
@@ -486,10 +494,13 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
                         for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + c0 + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8)
-                            *reinterpret_cast<uint4*>(out + c0 + e) =
-                                make_uint4(E::pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), E::pack(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])),
-                                           E::pack(__uint_as_float(x[e + 4]), __uint_as_float(x[e + 5])), E::pack(__uint_as_float(x[e + 6]), __uint_as_float(x[e + 7])));
+                        for (int e = 0; e < 32; e += 8) {
+                            uint32_t w[4], lo[4];
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) pack_split<F16>(__uint_as_float(x[e + 2 * y]), __uint_as_float(x[e + 2 * y + 1]), w[y], lo[y]);
+                            *reinterpret_cast<uint4*>(o + out_at + c0 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                            if (o_low) *reinterpret_cast<uint4*>(o_low + out_at + c0 + e) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        }
                     }
                 }
             }
@@ -516,45 +527,68 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
 
 #undef SA_ARRIVE
 
-// Joins the shares of a row: O = sum_s e^(lse_s - lse) O_s, a warp per row and head.  A share without keys has LSE -inf, and
-// its row need not be written.
+// Joins the shares of a row: O = sum_s e^(lse_s - lse) O_s.  `team` warps to a row and head, each with every team-th share; one
+// warp alone would wait for its chain of loads (17 us for 28 shares of 512 rows; a team of 8: 4 us).  A share without keys has
+// LSE -inf, and its row need not be written.
 template <int HD, bool F16>
-__global__ void __launch_bounds__(256) causal_join_kernel(const CParams p, int splits, const float* __restrict__ part_o, const float* __restrict__ part_lse,
-                                                         __nv_bfloat16* __restrict__ o, float* __restrict__ lse) {
-    using E = ptx::El<F16>;
+__global__ void __launch_bounds__(256) causal_join_kernel(const CParams p, int splits, int team, const float* __restrict__ part_o,
+                                                         const float* __restrict__ part_lse, __nv_bfloat16* __restrict__ o, __nv_bfloat16* __restrict__ o_low,
+                                                         float* __restrict__ lse) {
     constexpr int kPer = HD / 32;
+    __shared__ float sums[8][HD + 1];
     ptx::griddep_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t rows = (int64_t)p.B * p.H * p.Nq, at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (at >= rows) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, member = warp % team;
+    const int64_t rows = (int64_t)p.B * p.H * p.Nq, at = (int64_t)blockIdx.x * (8 / team) + warp / team;
     const int n = (int)(at % p.Nq), h = (int)(at / p.Nq % p.H), b = (int)(at / p.Nq / p.H);
-    if (p.cu_q != nullptr && (n < p.cu_q[0] || n >= p.cu_q[p.S])) return;       // (written where the shares are)
-    float top = -INFINITY;
-    for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_lse[s * rows + at]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc[kPer];
+    // (rows outside the sequences are written where the shares are)
+    const bool in = at < rows && (p.cu_q == nullptr || (n >= p.cu_q[0] && n < p.cu_q[p.S]));
+    float top = -INFINITY, sum = 0.f, acc[kPer];
 #pragma unroll
     for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        const float ls = part_lse[s * rows + at];
-        if (ls == -INFINITY) continue;
-        const float w = expf(ls - base);
-        sum += w;
-        const float* src = part_o + (s * rows + at) * HD + kPer * lane;
+    if (in) {
+        for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_lse[s * rows + at]);
 #pragma unroll
-        for (int e = 0; e < kPer; e += 2) {
-            const float2 x = *reinterpret_cast<const float2*>(src + e);
-            acc[e] = fmaf(w, x.x, acc[e]);
-            acc[e + 1] = fmaf(w, x.y, acc[e + 1]);
+        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+        for (int s = member; s < splits; s += team) {
+            const float ls = part_lse[s * rows + at];
+            const float* src = part_o + (s * rows + at) * HD + kPer * lane;
+            float x[kPer];
+#pragma unroll
+            for (int e = 0; e < kPer; e += 2) {
+                const float2 y = *reinterpret_cast<const float2*>(src + e);
+                x[e] = y.x;
+                x[e + 1] = y.y;
+            }
+            const float w = expf(ls - base);
+            sum += w;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) acc[e] = ls == -INFINITY ? acc[e] : fmaf(w, x[e], acc[e]);
         }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    __nv_bfloat16* dst = o + b * p.o.b + (int64_t)n * p.o.n + h * p.o.h + kPer * lane;
+    if (team > 1) {
 #pragma unroll
-    for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = E::pack(acc[e] * inv, acc[e + 1] * inv);
+        for (int e = 0; e < kPer; ++e) sums[warp][kPer * lane + e] = acc[e];
+        if (lane == 0) sums[warp][HD] = sum;
+        __syncthreads();
+        if (member != 0) return;
+        for (int y = 1; y < team; ++y) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) acc[e] += sums[warp + y][kPer * lane + e];
+            sum += sums[warp + y][HD];
+        }
+    }
+    if (!in) return;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t dst = b * p.o.b + (int64_t)n * p.o.n + h * p.o.h + kPer * lane;
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+        uint32_t w, low;
+        pack_split<F16>(acc[e] * inv, acc[e + 1] * inv, w, low);
+        *reinterpret_cast<uint32_t*>(o + dst + e) = w;
+        if (o_low) *reinterpret_cast<uint32_t*>(o_low + dst + e) = low;
+    }
     if (lane == 0) lse[at] = sum == 0.f ? -INFINITY : top + logf(sum);
 }
 
@@ -575,10 +609,13 @@ cudaError_t launch_behind(void (*kern)(Args...), unsigned grid, unsigned block, 
 }
 
 template <int HD>
-int launch_join(const CParams& p, bool f16, int splits, const float* part_o, const float* part_lse, void* o, float* lse, cudaStream_t st) {
-    const unsigned grid = (unsigned)(((int64_t)p.B * p.H * p.Nq + 7) / 8);
-    const cudaError_t e = f16 ? launch_behind(causal_join_kernel<HD, true>, grid, 256, 0, st, p, splits, part_o, part_lse, (__nv_bfloat16*)o, lse)
-                              : launch_behind(causal_join_kernel<HD, false>, grid, 256, 0, st, p, splits, part_o, part_lse, (__nv_bfloat16*)o, lse);
+int launch_join(const CParams& p, bool f16, int splits, const float* part_o, const float* part_lse, void* o, void* o_low, float* lse, cudaStream_t st) {
+    const int team = splits >= 24 ? 8 : splits >= 12 ? 4 : splits >= 4 ? 2 : 1, rows = 8 / team;
+    const unsigned grid = (unsigned)(((int64_t)p.B * p.H * p.Nq + rows - 1) / rows);
+    const cudaError_t e = f16 ? launch_behind(causal_join_kernel<HD, true>, grid, 256, 0, st, p, splits, team, part_o, part_lse, (__nv_bfloat16*)o,
+                                            (__nv_bfloat16*)o_low, lse)
+                              : launch_behind(causal_join_kernel<HD, false>, grid, 256, 0, st, p, splits, team, part_o, part_lse, (__nv_bfloat16*)o,
+                                            (__nv_bfloat16*)o_low, lse);
     host::count_launches(1);
     return e == cudaSuccess ? SA_OK : SA_ERR_LAUNCH;
 }
@@ -622,7 +659,8 @@ inline FwdPlan plan_fwd(const CParams& c) {
 }
 
 template <int HD, bool F16>
-int launch_fwd_tc(const CParams& c, const void* q, const void* k, const void* v, void* o, float* lse, uint8_t* ws, DeviceStatus* status, cudaStream_t st) {
+int launch_fwd_tc(const CParams& c, const void* q, const void* k, const void* v, void* o, void* o_low, float* lse, uint8_t* ws, DeviceStatus* status,
+                  cudaStream_t st) {
     const FwdPlan f = plan_fwd(c);
     if (f.items * c.H * f.splits > 0x3fffffff) return SA_ERR_UNSUPPORTED;
     CUtensorMap mq, mk, mv;
@@ -653,10 +691,10 @@ int launch_fwd_tc(const CParams& c, const void* q, const void* k, const void* v,
     }
     const int64_t units = f.items * c.H * f.splits;
     const unsigned grid = (unsigned)(units < host::sm_count() ? units : host::sm_count());
-    kern<<<grid, kFwdThreads, FwdLayout<HD>::kBytes, st>>>(P, mq, mk, mv, (__nv_bfloat16*)o, lse);
+    kern<<<grid, kFwdThreads, FwdLayout<HD>::kBytes, st>>>(P, mq, mk, mv, (__nv_bfloat16*)o, (__nv_bfloat16*)o_low, lse);
     host::count_launches(1);
     if (cudaGetLastError() != cudaSuccess) return SA_ERR_LAUNCH;
-    return f.splits > 1 ? launch_join<HD>(c, F16, f.splits, P.part_o, P.part_lse, o, lse, st) : SA_OK;
+    return f.splits > 1 ? launch_join<HD>(c, F16, f.splits, P.part_o, P.part_lse, o, o_low, lse, st) : SA_OK;
 }
 
 }  // namespace causal

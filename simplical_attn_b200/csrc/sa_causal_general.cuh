@@ -121,15 +121,21 @@ __device__ __forceinline__ void accumulate(float (&acc)[R][GenShape<DP>::kDpt], 
     }
 }
 
+// (with `low`: what rounding took, too)
 template <typename T, int DP>
-__device__ __forceinline__ void store_row(T* row, const float (&v)[GenShape<DP>::kDpt], float f, int tx, int D) {
+__device__ __forceinline__ void store_row(T* row, const float (&v)[GenShape<DP>::kDpt], float f, int tx, int D, T* low = nullptr) {
     using L = GenShape<DP>;
 #pragma unroll
     for (int g = 0; g < L::kDpt / L::kVec; ++g)
 #pragma unroll
         for (int e = 0; e < L::kVec; ++e) {
             const int d = 16 * L::kVec * g + L::kVec * tx + e;
-            if (d < D) row[d] = from_f<T>(v[g * L::kVec + e] * f);
+            if (d < D) {
+                const float x = v[g * L::kVec + e] * f;
+                const T t = from_f<T>(x);
+                row[d] = t;
+                if (low) low[d] = from_f<T>(x - to_f<T>(t));
+            }
         }
 }
 
@@ -146,7 +152,8 @@ __device__ __forceinline__ float half_sum(float v) {
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kGenThreads) causal_fwd_kernel(const CParams p, const T* __restrict__ q, const T* __restrict__ k,
-                                                                const T* __restrict__ v, T* __restrict__ o, float* __restrict__ lse, int blocks_q) {
+                                                                const T* __restrict__ v, T* __restrict__ o, T* __restrict__ o_low, float* __restrict__ lse,
+                                                                int blocks_q) {
     using L = GenShape<DP>;
     extern __shared__ float4 smem4[];
     float* const qt = reinterpret_cast<float*>(smem4);
@@ -161,6 +168,7 @@ __global__ void __launch_bounds__(kGenThreads) causal_fwd_kernel(const CParams p
     k += s.b * p.k.b + s.k0 * p.k.n + h / p.G * p.k.h;
     v += s.b * p.v.b + s.k0 * p.v.n + h / p.G * p.v.h;
     o += s.b * p.o.b + s.q0 * p.o.n + h * p.o.h;
+    if (o_low) o_low += s.b * p.o.b + s.q0 * p.o.n + h * p.o.h;
     lse += ((int64_t)s.b * p.H + h) * p.Nq + s.q0;
 
     for (int i0 = blk * kGenRows; i0 < s.nq; i0 += blocks_q * kGenRows) {
@@ -216,7 +224,7 @@ __global__ void __launch_bounds__(kGenThreads) causal_fwd_kernel(const CParams p
             const float sum = half_sum(l[r]);
             if (i < s.nq) {
                 const bool none = i + s.off() < 0;
-                store_row<T, DP>(o + (int64_t)i * p.o.n, acc[r], none ? 0.f : 1.f / sum, tx, p.D);
+                store_row<T, DP>(o + (int64_t)i * p.o.n, acc[r], none ? 0.f : 1.f / sum, tx, p.D, o_low ? o_low + (int64_t)i * p.o.n : nullptr);
                 if (tx == 0) lse[i] = none ? -INFINITY : m[r] + logf(sum);
             }
         }
@@ -229,15 +237,16 @@ __global__ void __launch_bounds__(kGenThreads) causal_fwd_kernel(const CParams p
 
 // Delta = sum_d dO O of every row, a warp per row and head.
 template <typename T>
-__global__ void __launch_bounds__(256) causal_delta_kernel(const CParams p, const T* __restrict__ o, const T* __restrict__ d_o, float* __restrict__ delta) {
+__global__ void __launch_bounds__(256) causal_delta_kernel(const CParams p, const T* __restrict__ o, const T* __restrict__ o_low, const T* __restrict__ d_o,
+                                                          float* __restrict__ delta) {
     const int lane = threadIdx.x & 31;
     const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (w >= (int64_t)p.B * p.Nq * p.H) return;
     const int h = (int)(w % p.H), i = (int)(w / p.H % p.Nq), b = (int)(w / p.H / p.Nq);
-    o += b * p.o.b + i * p.o.n + h * p.o.h;
+    const int64_t at = b * p.o.b + i * p.o.n + h * p.o.h;
     d_o += b * p.d_o.b + i * p.d_o.n + h * p.d_o.h;
     float sum = 0.f;
-    for (int d = lane; d < p.D; d += 32) sum = fmaf(to_f<T>(o[d]), to_f<T>(d_o[d]), sum);
+    for (int d = lane; d < p.D; d += 32) sum = fmaf(to_f<T>(o[at + d]) + (o_low ? to_f<T>(o_low[at + d]) : 0.f), to_f<T>(d_o[d]), sum);
     sum = warp_sum(sum);
     if (lane == 0) delta[((int64_t)b * p.H + h) * p.Nq + i] = sum;
 }
@@ -393,37 +402,37 @@ __global__ void __launch_bounds__(kGenThreads) causal_dkv_kernel(const CParams p
 }
 
 template <typename T, int DP>
-int launch_general_fwd_d(const CParams& p, const void* q, const void* k, const void* v, void* o, float* lse, cudaStream_t st) {
+int launch_general_fwd_d(const CParams& p, const void* q, const void* k, const void* v, void* o, void* o_low, float* lse, cudaStream_t st) {
     using L = GenShape<DP>;
     const int bq = ceil_div(p.max_q, kGenRows);
     const int64_t grid = (int64_t)bq * p.H * p.S;
     if (grid > 0x7fffffff) return SA_ERR_UNSUPPORTED;
     auto kern = causal_fwd_kernel<T, DP>;
     if (!allow_dynamic_smem((const void*)kern, L::kFwdBytes)) return SA_ERR_LAUNCH;
-    kern<<<(unsigned)grid, kGenThreads, L::kFwdBytes, st>>>(p, (const T*)q, (const T*)k, (const T*)v, (T*)o, lse, bq);
+    kern<<<(unsigned)grid, kGenThreads, L::kFwdBytes, st>>>(p, (const T*)q, (const T*)k, (const T*)v, (T*)o, (T*)o_low, lse, bq);
     host::count_launches(1);
     return cudaGetLastError() == cudaSuccess ? SA_OK : SA_ERR_LAUNCH;
 }
 
 template <typename T>
-int launch_delta(const CParams& p, const void* o, const void* d_o, float* delta, cudaStream_t st) {
+int launch_delta(const CParams& p, const void* o, const void* o_low, const void* d_o, float* delta, cudaStream_t st) {
     const int64_t rows = (int64_t)p.B * p.Nq * p.H;
     if (rows / 8 + 1 > 0x7fffffff) return SA_ERR_UNSUPPORTED;
-    causal_delta_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, (const T*)o, (const T*)d_o, delta);
+    causal_delta_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, (const T*)o, (const T*)o_low, (const T*)d_o, delta);
     host::count_launches(1);
     return cudaGetLastError() == cudaSuccess ? SA_OK : SA_ERR_LAUNCH;
 }
 
 template <typename T, int DP>
-int launch_general_bwd_d(const CParams& p, const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, void* dq,
-                         void* dk, void* dv, float* delta, cudaStream_t st) {
+int launch_general_bwd_d(const CParams& p, const void* q, const void* k, const void* v, const void* o, const void* o_low, const float* lse, const void* d_o,
+                         void* dq, void* dk, void* dv, float* delta, cudaStream_t st) {
     using L = GenShape<DP>;
     const int bq = ceil_div(p.max_q, kGenRows), bk = ceil_div(p.max_k, L::kCols);
     const int64_t gq = (int64_t)bq * p.H * p.S, gk = (int64_t)bk * p.Hkv * p.S;
     if (gq > 0x7fffffff || gk > 0x7fffffff) return SA_ERR_UNSUPPORTED;
     if (!allow_dynamic_smem((const void*)causal_dq_kernel<T, DP>, L::kDqBytes) || !allow_dynamic_smem((const void*)causal_dkv_kernel<T, DP>, L::kDkvBytes))
         return SA_ERR_LAUNCH;
-    const int rc = launch_delta<T>(p, o, d_o, delta, st);
+    const int rc = launch_delta<T>(p, o, o_low, d_o, delta, st);
     if (rc != SA_OK) return rc;
     if (dq) {
         causal_dq_kernel<T, DP><<<(unsigned)gq, kGenThreads, L::kDqBytes, st>>>(p, (const T*)q, (const T*)k, (const T*)v, lse, delta, (const T*)d_o, (T*)dq, bq);

@@ -83,15 +83,16 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         }
     const int h0 = ((int)hb - first_block) * kHeads, nh = min(kHeads, heads - h0);
 
-    // the two vectors of this group within a head
+    // the two vectors of this group within a head, half of the turned (or of the other) elements apart, so that neighbouring
+    // threads read neighbouring vectors: the partners of half-split pairs, or V / 2 interleaved pairs each
     const bool turned = g < p.turned_groups;
     int oa, ob;
     if (!turned) {
-        oa = p.rd + (int)(g - p.turned_groups) * 2 * V;
-        ob = oa + V;
-    } else if (INTERLEAVED) {
-        oa = (int)g * 2 * V;
-        ob = oa + V;
+        oa = p.rd + (int)(g - p.turned_groups) * V;
+        ob = oa + (int)(p.groups - p.turned_groups) * V;
+    } else if (INTERLEAVED && V == 1) {
+        oa = 2 * (int)g;
+        ob = oa + 1;
     } else {
         oa = (int)g * V;
         ob = p.rd / 2 + oa;
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         float cs[V], sn[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const int i = (int)g * V + e;
+            const int i = !INTERLEAVED || V == 1 ? (int)g * V + e : (e < V / 2 ? oa : ob) / 2 + e % (V / 2 ? V / 2 : 1);
             const double f = p.frequency_bits == 64 ? ((const double*)p.frequencies)[i] : (double)((const float*)p.frequencies)[i];
             cos_sin_quarters(quarters * f, cs[e], sn[e]);
             cs[e] *= p.magnitude;

@@ -352,8 +352,12 @@ def test_calls_through_ctypes_and_traces(monkeypatch):
     assert all(torch.equal(plain[n], got[n]) for n in plain)
     traced = torch.jit.trace(lambda a, b, c: sab.causal_attention(a, b, c, cu_q=cu_q, cu_k=cu_k), (q, k, v), check_trace=False)
     assert torch.equal(traced(q, k, v), plain["o"])
+    o, lse, low = sab.causal_attention_fwd(q, k, v, 0.125, cu_q, cu_k, low=True)
+    bw = sab.causal_attention_bwd(q, k, v, o, lse, d_o, 0.125, cu_q, cu_k, need=(True, False, True), o_low=low)
     fw = sab.causal_attention_fwd(q, k, v, 0.125, cu_q, cu_k)
-    bw = sab.causal_attention_bwd(q, k, v, *fw, d_o, 0.125, cu_q, cu_k, need=(True, False, True))
+    assert torch.equal(fw[0], o) and torch.equal(fw[1], lse) and len(fw) == 2
+    with pytest.raises(ValueError, match="o_low"):
+        sab.causal_attention_bwd(q, k, v, o, lse, d_o, 0.125, cu_q, cu_k, o_low=low[:50])
     assert torch.equal(fw[0], plain["o"]) and torch.equal(bw[0], plain["dq"]) and bw[1] is None and torch.equal(bw[2], plain["dv"])
 
 
@@ -417,8 +421,8 @@ def test_entries_validate():
     lib = _abi.load()
     assert ctypes.sizeof(_abi.CausalParams) == 12 * 4 + 8 * 24
     nul, some = ctypes.c_void_p(0), ctypes.c_void_p(4096)
-    fwd = lambda p, a=nul, ws=nul, n=0, status=some: lib.sa_causal_forward(p, *[a] * 5, nul, nul, ws, n, status, nul)
-    bwd = lambda p, a=nul, ws=nul, n=0, status=some: lib.sa_causal_backward(p, *[a] * 9, nul, nul, ws, n, status, nul)
+    fwd = lambda p, a=nul, ws=nul, n=0, status=some: lib.sa_causal_forward(p, *[a] * 4, nul, a, nul, nul, ws, n, status, nul)
+    bwd = lambda p, a=nul, ws=nul, n=0, status=some: lib.sa_causal_backward(p, *[a] * 4, nul, *[a] * 5, nul, nul, ws, n, status, nul)
     for call in (fwd, bwd):
         assert call(None) == 1 and call(params()) == 1
         for bad in (dict(B=0), dict(Nq=0), dict(Nk=-1), dict(H=5), dict(Hkv=0), dict(D=0), dict(sequences=-1), dict(max_q=-1),
