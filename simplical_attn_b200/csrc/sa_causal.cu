@@ -46,7 +46,7 @@ CParams make_params(const sa_causal_params* p, const int32_t* cu_q, const int32_
 
 // Whether the tensor-core kernels cover the problem (pointers and what a tensor map can hold are looked at in the call).
 bool tc_ok(const sa_causal_params* p, bool backward) {
-    if (p->dtype == SA_F32 || (p->D != 64 && p->D != 128)) return false;
+    if (p->dtype == SA_F32 || p->D > 128 || p->D % 8 != 0) return false;
     if (!(p->scale > 0.f)) return false;            // the row maximum is taken before scaling
     const CParams c = make_params(p, nullptr, nullptr);
     for (const sa_strides* s : {&c.q, &c.k, &c.v, &c.o})
@@ -72,15 +72,12 @@ CParams planned(const sa_causal_params* p) {
     return make_params(p, cu, cu);
 }
 
-// f(head dim, element type) of the tensor-core kernels
+// f(columns of a tile, element type) of the tensor-core kernels
 template <typename F>
 int dispatch_tc(const sa_causal_params* p, F&& f) {
     auto by_type = [&](auto d) { return p->dtype == SA_F16 ? f(d, std::true_type{}) : f(d, std::false_type{}); };
-    return p->D == 128 ? by_type(std::integral_constant<int, 128>{}) : by_type(std::integral_constant<int, 64>{});
+    return tile_columns(p->D) == 128 ? by_type(std::integral_constant<int, 128>{}) : by_type(std::integral_constant<int, 64>{});
 }
-
-size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
-size_t delta_bytes(const sa_causal_params* p) { return align256((size_t)p->B * p->H * p->Nq * sizeof(float)); }
 
 bool workspace_ok(const void* ws, size_t bytes, size_t need) {
     if (need == 0) return true;
@@ -97,14 +94,21 @@ size_t sa_causal_forward_workspace_size(const sa_causal_params* p) {
     using namespace sa::causal;
     if (validate(p) != SA_OK) return 0;
     const int algo = resolve(p, false);
-    return algo == SA_ALGO_TCGEN05 ? plan_fwd(planned(p)).bytes : algo == SA_CAUSAL_FEW_ROWS ? plan_few(planned(p)).bytes : 0;
+    if (algo < 0) return 0;
+    // (a call whose pointers or strides turn out not to suit the tensor cores takes the general kernels)
+    const CParams c = planned(p);
+    const size_t general = plan_general(c, false).bytes, own = algo == SA_ALGO_TCGEN05 ? plan_fwd(c).bytes : algo == SA_CAUSAL_FEW_ROWS ? plan_few(c).bytes : 0;
+    return general > own ? general : own;
 }
 
 size_t sa_causal_backward_workspace_size(const sa_causal_params* p) {
     using namespace sa::causal;
     if (validate(p) != SA_OK) return 0;
-    if (resolve(p, true) != SA_ALGO_TCGEN05) return delta_bytes(p);
-    return plan_bwd(planned(p)).bytes;
+    const int algo = resolve(p, true);
+    if (algo < 0) return 0;
+    const CParams c = planned(p);
+    const size_t general = plan_general(c, true).bytes, own = algo == SA_ALGO_TCGEN05 ? plan_bwd(c).bytes : 0;
+    return general > own ? general : own;
 }
 
 int sa_causal_resolve(const sa_causal_params* p, int backward) {
@@ -137,7 +141,7 @@ int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, c
         // (BAD_STRIDE: nothing has been launched)
         if (rc != SA_ERR_BAD_STRIDE || p->algo == SA_ALGO_TCGEN05) return rc;
     }
-    return dispatch_general(p->dtype, p->D, [&](auto t, auto d) { return launch_general_fwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, o_low, lse, st); });
+    return dispatch_general(p->dtype, p->D, [&](auto t, auto d) { return launch_general_fwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, o_low, lse, static_cast<uint8_t*>(workspace), st); });
 }
 
 int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, const void* v, const void* o, const void* o_low, const float* lse,
@@ -152,7 +156,6 @@ int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, 
     const int algo = resolve(p, true);
     if (algo < 0) return -algo;
     const CParams c = make_params(p, p->sequences > 0 ? cu_q : nullptr, p->sequences > 0 ? cu_k : nullptr);
-    float* delta = static_cast<float*>(workspace);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (algo == SA_ALGO_TCGEN05) {
         if (sa::host::cc_major() != 10) return SA_ERR_NOT_SM100;
@@ -167,7 +170,7 @@ int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, 
         if (rc != SA_ERR_BAD_STRIDE || p->algo == SA_ALGO_TCGEN05) return rc;
     }
     return dispatch_general(p->dtype, p->D, [&](auto t, auto d) {
-        return launch_general_bwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, o_low, lse, d_o, dq, dk, dv, delta, st);
+        return launch_general_bwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, o_low, lse, d_o, dq, dk, dv, static_cast<uint8_t*>(workspace), st);
     });
 }
 

@@ -20,6 +20,9 @@ struct CParams {
     sa_strides q, k, v, o, d_o, dq, dk, dv;
 };
 
+// Columns of the tensor-core kernels' tiles: the head dim, filled up with zeros by the loads.
+inline int tile_columns(int D) { return D <= 64 ? 64 : 128; }
+
 // Rows of one sequence: queries [q0, q0 + nq) and keys [k0, k0 + nk) of batch element b.  Query i (from 0) sees keys
 // j <= i + off, off = nk - nq.
 struct Seq {
@@ -66,6 +69,22 @@ __device__ __forceinline__ void empty_lse_outside(float* lse, int H, int n, cons
 }
 
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Shares that the walks of `units` units, of `steps` steps each at most, are cut into: one where the units fill the
+// multiprocessors, else what makes rounds of units times their steps least.  `around` is what a unit costs besides its steps and
+// `joining` what adding up the shares costs, in steps.
+inline int plan_shares(int64_t units, int steps, int sms, int most, int around, int joining) {
+    int shares = 1;
+    int64_t best = (units + sms - 1) / sms * (steps + around);
+    for (int s = 2; s <= most && s <= steps && units * (s - 1) < 2 * sms; ++s) {
+        const int64_t cost = (units * s + sms - 1) / sms * (ceil_div(steps, s) + around) + joining;
+        if (cost < best) {
+            best = cost;
+            shares = s;
+        }
+    }
+    return shares;
+}
 
 }  // namespace causal
 }  // namespace sa

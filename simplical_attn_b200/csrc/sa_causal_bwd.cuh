@@ -1,4 +1,4 @@
-// Causal attention backward on the sm_100a tensor cores (bf16 / fp16, head dim 64 and 128).
+// Causal attention backward on the sm_100a tensor cores (bf16 / fp16; head dims as in the forward).
 //
 //     Delta_i = sum_d dO_id O_id,   P = exp(S - LSE),   dS = scale P (dO V^T - Delta),
 //     dV = P^T dO,   dK = dS^T Q,   dQ = dS K.
@@ -53,8 +53,10 @@ __global__ void __launch_bounds__(256) causal_delta16_kernel(const CParams p, co
         i = (int)(w / p.H % p.Nq);
         b = (int)(w / p.H / p.Nq);
         const int64_t at = b * p.o.b + i * p.o.n + h * p.o.h + 8 * lane;
-        const uint4 x = *reinterpret_cast<const uint4*>(o + at), z = o_low ? *reinterpret_cast<const uint4*>(o_low + at) : make_uint4(0, 0, 0, 0);
-        const uint4 y = *reinterpret_cast<const uint4*>(d_o + b * p.d_o.b + i * p.d_o.n + h * p.d_o.h + 8 * lane);
+        const uint4 none = make_uint4(0, 0, 0, 0);
+        const bool col = 8 * lane < p.D;
+        const uint4 x = col ? *reinterpret_cast<const uint4*>(o + at) : none, z = col && o_low ? *reinterpret_cast<const uint4*>(o_low + at) : none;
+        const uint4 y = col ? *reinterpret_cast<const uint4*>(d_o + b * p.d_o.b + i * p.d_o.n + h * p.d_o.h + 8 * lane) : none;
         const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w}, zw[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -452,9 +454,10 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
-                        *reinterpret_cast<uint4*>(dst + c0 + e) =
-                            make_uint4(E::pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), E::pack(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])),
-                                       E::pack(__uint_as_float(x[e + 4]), __uint_as_float(x[e + 5])), E::pack(__uint_as_float(x[e + 6]), __uint_as_float(x[e + 7])));
+                        if (c0 + e < p.D)
+                            *reinterpret_cast<uint4*>(dst + c0 + e) =
+                                make_uint4(E::pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), E::pack(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])),
+                                           E::pack(__uint_as_float(x[e + 4]), __uint_as_float(x[e + 5])), E::pack(__uint_as_float(x[e + 6]), __uint_as_float(x[e + 7])));
                 }
             }
             if (u.n > 0) {
@@ -464,8 +467,8 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
         }
     }
     if (p.cu_k != nullptr && P.splits == 1) {
-        if (dk) zero_outside(dk, p.dk, p.Hkv, HD, p.Nk, p.cu_k, p.S, blockIdx.x, gridDim.x);
-        if (dv) zero_outside(dv, p.dv, p.Hkv, HD, p.Nk, p.cu_k, p.S, blockIdx.x, gridDim.x);
+        if (dk) zero_outside(dk, p.dk, p.Hkv, p.D, p.Nk, p.cu_k, p.S, blockIdx.x, gridDim.x);
+        if (dv) zero_outside(dv, p.dv, p.Hkv, p.D, p.Nk, p.cu_k, p.S, blockIdx.x, gridDim.x);
     }
     tc_fence_before();
     __syncthreads();
@@ -829,9 +832,10 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
-                        *reinterpret_cast<uint4*>(dst + c0 + e) =
-                            make_uint4(E::pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), E::pack(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])),
-                                       E::pack(__uint_as_float(x[e + 4]), __uint_as_float(x[e + 5])), E::pack(__uint_as_float(x[e + 6]), __uint_as_float(x[e + 7])));
+                        if (col + c0 + e < p.D)
+                            *reinterpret_cast<uint4*>(dst + c0 + e) =
+                                make_uint4(E::pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), E::pack(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])),
+                                           E::pack(__uint_as_float(x[e + 4]), __uint_as_float(x[e + 5])), E::pack(__uint_as_float(x[e + 6]), __uint_as_float(x[e + 7])));
                 }
             }
             if (u.n > 0) {
@@ -840,7 +844,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
             }
         }
     }
-    if (p.cu_q != nullptr && P.splits == 1) zero_outside(dq, p.dq, p.H, HD, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
+    if (p.cu_q != nullptr && P.splits == 1) zero_outside(dq, p.dq, p.H, p.D, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
     tc_fence_before();
     __syncthreads();
     if (warp == 8) {
@@ -854,11 +858,12 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
 // Adds the shares of a gradient in their order: [splits][B][heads][n][D] fp32 -> rows (b, i, h); a thread takes 4 columns.
 template <int HD, bool F16>
 __global__ void __launch_bounds__(256) causal_add_kernel(const float* __restrict__ part, __nv_bfloat16* __restrict__ out, sa_strides so, int splits, int B,
-                                                        int heads, int n, const int* cu, int S) {
+                                                        int heads, int n, int D, const int* cu, int S) {
     using E = ptx::El<F16>;
     const int64_t rows = (int64_t)B * heads * n, idx = (int64_t)blockIdx.x * 256 + threadIdx.x, at = idx / (HD / 4);
-    if (at >= rows) return;
-    const int c = (int)(idx % (HD / 4)) * 4, i = (int)(at % n), h = (int)(at / n % heads), b = (int)(at / n / heads);
+    const int c = (int)(idx % (HD / 4)) * 4;
+    if (at >= rows || c >= D) return;
+    const int i = (int)(at % n), h = (int)(at / n % heads), b = (int)(at / n / heads);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (cu == nullptr || (i >= cu[0] && i < cu[S])) {         // (rows outside every sequence: zeros)
 #pragma unroll 4
@@ -874,26 +879,13 @@ __global__ void __launch_bounds__(256) causal_add_kernel(const float* __restrict
 }
 
 template <int HD>
-int launch_add(bool f16, const float* part, void* out, const sa_strides& so, int splits, int B, int heads, int n, const int* cu, int S, cudaStream_t st) {
+int launch_add(bool f16, const float* part, void* out, const sa_strides& so, int splits, int B, int heads, int n, int D, const int* cu, int S,
+               cudaStream_t st) {
     const unsigned grid = (unsigned)(((int64_t)B * heads * n * (HD / 4) + 255) / 256);
-    if (f16) causal_add_kernel<HD, true><<<grid, 256, 0, st>>>(part, (__nv_bfloat16*)out, so, splits, B, heads, n, cu, S);
-    else causal_add_kernel<HD, false><<<grid, 256, 0, st>>>(part, (__nv_bfloat16*)out, so, splits, B, heads, n, cu, S);
+    if (f16) causal_add_kernel<HD, true><<<grid, 256, 0, st>>>(part, (__nv_bfloat16*)out, so, splits, B, heads, n, D, cu, S);
+    else causal_add_kernel<HD, false><<<grid, 256, 0, st>>>(part, (__nv_bfloat16*)out, so, splits, B, heads, n, D, cu, S);
     host::count_launches(1);
     return cudaGetLastError() == cudaSuccess ? SA_OK : SA_ERR_LAUNCH;
-}
-
-// Shares of a unit's walk of `steps` steps: where the units do not fill the multiprocessors (see plan_fwd).
-inline int plan_shares(int64_t units, int steps, int sms) {
-    int shares = 1;
-    int64_t best = (units + sms - 1) / sms * (steps + 2);
-    for (int s = 2; s <= 16 && 2 * s <= steps && units * (s - 1) < 2 * sms; ++s) {
-        const int64_t cost = (units * s + sms - 1) / sms * (ceil_div(steps, s) + 2) + 4;
-        if (cost < best) {
-            best = cost;
-            shares = s;
-        }
-    }
-    return shares;
 }
 
 struct BwdPlan {
@@ -907,16 +899,16 @@ inline BwdPlan plan_bwd(const CParams& c) {
     f.items_q = packed ? list_capacity(c.Nq, kTile, c.S) : (int64_t)ceil_div(c.Nq, kTile) * c.S;
     f.items_k = packed ? list_capacity(c.Nk, kTile, c.S) : (int64_t)ceil_div(c.Nk, kTile) * c.S;
     const int sms = host::sm_count();
-    f.splits_q = plan_shares(f.items_q * c.H, ceil_div(c.max_k, kTile), sms);
-    f.splits_k = plan_shares(f.items_k * c.Hkv, (int)((int64_t)ceil_div(c.max_q, kTile) * c.G < (1 << 20) ? ceil_div(c.max_q, kTile) * c.G : 1 << 20), sms);
+    f.splits_q = plan_shares(f.items_q * c.H, ceil_div(c.max_k, kTile), sms, 16, 2, 4);
+    f.splits_k = plan_shares(f.items_k * c.Hkv, (int)((int64_t)ceil_div(c.max_q, kTile) * c.G < (1 << 20) ? ceil_div(c.max_q, kTile) * c.G : 1 << 20), sms, 16, 2, 4);
     size_t at = 0;
     auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };
     f.delta = take((size_t)c.B * c.H * c.Nq * 4);
     f.list_q = take(packed ? list_bytes(f.items_q) : 0);
     f.list_k = take(packed ? list_bytes(f.items_k) : 0);
-    f.part_q = take(f.splits_q > 1 ? (size_t)f.splits_q * c.B * c.H * c.Nq * c.D * 4 : 0);
-    f.part_k = take(f.splits_k > 1 ? (size_t)f.splits_k * c.B * c.Hkv * c.Nk * c.D * 4 : 0);
-    f.part_v = take(f.splits_k > 1 ? (size_t)f.splits_k * c.B * c.Hkv * c.Nk * c.D * 4 : 0);
+    f.part_q = take(f.splits_q > 1 ? (size_t)f.splits_q * c.B * c.H * c.Nq * tile_columns(c.D) * 4 : 0);
+    f.part_k = take(f.splits_k > 1 ? (size_t)f.splits_k * c.B * c.Hkv * c.Nk * tile_columns(c.D) * 4 : 0);
+    f.part_v = take(f.splits_k > 1 ? (size_t)f.splits_k * c.B * c.Hkv * c.Nk * tile_columns(c.D) * 4 : 0);
     f.bytes = at;
     return f;
 }
@@ -927,8 +919,8 @@ int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v,
     const BwdPlan f = plan_bwd(c);
     if (f.items_q * c.H * f.splits_q > 0x3fffffff || f.items_k * c.Hkv * f.splits_k > 0x3fffffff) return SA_ERR_UNSUPPORTED;
     CUtensorMap mq, mk, mv, mo;
-    if (!host::make_map(&mq, q, c.B, c.Nq, c.H, HD, c.q, kTile, F16) || !host::make_map(&mk, k, c.B, c.Nk, c.Hkv, HD, c.k, kTile, F16) ||
-        !host::make_map(&mv, v, c.B, c.Nk, c.Hkv, HD, c.v, kTile, F16) || !host::make_map(&mo, d_o, c.B, c.Nq, c.H, HD, c.d_o, kTile, F16))
+    if (!host::make_map(&mq, q, c.B, c.Nq, c.H, c.D, c.q, kTile, F16) || !host::make_map(&mk, k, c.B, c.Nk, c.Hkv, c.D, c.k, kTile, F16) ||
+        !host::make_map(&mv, v, c.B, c.Nk, c.Hkv, c.D, c.v, kTile, F16) || !host::make_map(&mo, d_o, c.B, c.Nq, c.H, c.D, c.d_o, kTile, F16))
         return SA_ERR_BAD_STRIDE;
     if (!allow_dynamic_smem((const void*)causal_dkv_tc_kernel<HD, F16>, ColLayout<HD>::kBytes) ||
         !allow_dynamic_smem((const void*)causal_dq_tc_kernel<HD, F16>, RowLayout<HD>::kBytes))
@@ -971,8 +963,8 @@ int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v,
             P, mq, mk, mv, mo, (__nv_bfloat16*)dk, (__nv_bfloat16*)dv);
         host::count_launches(1);
         if (f.splits_k > 1) {
-            if (dk) rc = launch_add<HD>(F16, P.part0, dk, c.dk, f.splits_k, c.B, c.Hkv, c.Nk, c.cu_k, c.S, st);
-            if (dv && rc == SA_OK) rc = launch_add<HD>(F16, P.part1, dv, c.dv, f.splits_k, c.B, c.Hkv, c.Nk, c.cu_k, c.S, st);
+            if (dk) rc = launch_add<HD>(F16, P.part0, dk, c.dk, f.splits_k, c.B, c.Hkv, c.Nk, c.D, c.cu_k, c.S, st);
+            if (dv && rc == SA_OK) rc = launch_add<HD>(F16, P.part1, dv, c.dv, f.splits_k, c.B, c.Hkv, c.Nk, c.D, c.cu_k, c.S, st);
         }
     }
     if (dq && rc == SA_OK) {
@@ -984,7 +976,7 @@ int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v,
         const int64_t units = f.items_q * c.H * f.splits_q;
         causal_dq_tc_kernel<HD, F16><<<(unsigned)(units < sms ? units : sms), kBwdThreads, RowLayout<HD>::kBytes, st>>>(P, mq, mk, mv, mo, (__nv_bfloat16*)dq);
         host::count_launches(1);
-        if (f.splits_q > 1) rc = launch_add<HD>(F16, P.part0, dq, c.dq, f.splits_q, c.B, c.H, c.Nq, c.cu_q, c.S, st);
+        if (f.splits_q > 1) rc = launch_add<HD>(F16, P.part0, dq, c.dq, f.splits_q, c.B, c.H, c.Nq, c.D, c.cu_q, c.S, st);
     }
     if (rc != SA_OK) return rc;
     return cudaGetLastError() == cudaSuccess ? SA_OK : SA_ERR_LAUNCH;

@@ -1,4 +1,5 @@
-// Causal attention of a few queries over many keys (single tokens, a handful of drafted ones), bf16 / fp16, head dim 64 and 128.
+// Causal attention of a few queries over many keys (single tokens, a handful of drafted ones), bf16 / fp16, head dims up to
+// 128 that are multiples of 8 (tiles of 64 or 128 columns, filled up with zeros).
 //
 // K and V are read once and little is computed with them: HBM bandwidth bounds it, latency where they are short.  The rows of
 // a block are the queries of all heads that share a KV head (query i, head g of the group: row i G + g), 16 or 32 of them, so a
@@ -112,10 +113,10 @@ causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __re
                 for (int e = 0; e < 16 * kChunks / 32; ++e) {
                     const int c = lane + 32 * e, row = c / kChunks, ch = c % kChunks, j = j0 + row;
                     const uint32_t at = st + row * HD * 2 + ((ch ^ (row & 7)) << 4);
-                    const bool in = j < c1;
-                    const int64_t jj = in ? j : c0;
-                    cp16(at, kh + jj * p.k.n + ch * 8, in);               // rows behind the share: zeros
-                    cp16(at + L::kHalf, vh + jj * p.v.n + ch * 8, in);
+                    const bool in = j < c1 && ch * 8 < p.D;
+                    const int64_t jj = in ? j : c0, cc = in ? ch * 8 : 0;
+                    cp16(at, kh + jj * p.k.n + cc, in);                   // rows behind the share: zeros
+                    cp16(at + L::kHalf, vh + jj * p.v.n + cc, in);
                 }
             }
             cp_commit();
@@ -128,7 +129,7 @@ causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __re
         for (int c = tid; c < 16 * MT * kChunks; c += kFewThreads) {
             const int row = c / kChunks, ch = c % kChunks, rho = r0 + row;
             uint4 w = make_uint4(0, 0, 0, 0);
-            if (rho < R) {
+            if (rho < R && ch * 8 < p.D) {
                 const int i = rho / p.G, g = rho - i * p.G;
                 w = *reinterpret_cast<const uint4*>(q + s.b * p.q.b + (int64_t)(s.q0 + i) * p.q.n + (hk * p.G + g) * p.q.h + ch * 8);
             }
@@ -325,7 +326,7 @@ causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __re
             if (P.shares > 1) {
                 if (!none) *reinterpret_cast<float4*>(P.part_o + (share * rows_all + at) * HD + d) = make_float4(t.x * inv, t.y * inv, t.z * inv, t.w * inv);
                 if (d == 0) P.part_lse[share * rows_all + at] = ll;
-            } else {
+            } else if (d < p.D) {
                 const int64_t dst = s.b * p.o.b + (int64_t)(s.q0 + i) * p.o.n + h * p.o.h + d;
                 uint2 y, low;
                 pack_split<F16>(t.x * inv, t.y * inv, y.x, low.x);
@@ -338,7 +339,7 @@ causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __re
         __syncthreads();
     }
     if (p.cu_q != nullptr) {
-        zero_outside(o, p.o, p.H, HD, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
+        zero_outside(o, p.o, p.H, p.D, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
         empty_lse_outside(lse, p.H, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
     }
 }
@@ -377,7 +378,7 @@ inline FewPlan plan_few(const CParams& c) {
     const size_t all = (size_t)c.B * c.H * c.Nq;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };
-    f.part_o = take(f.shares > 1 ? (size_t)f.shares * all * c.D * 4 : 0);
+    f.part_o = take(f.shares > 1 ? (size_t)f.shares * all * tile_columns(c.D) * 4 : 0);
     f.part_lse = take(f.shares > 1 ? (size_t)f.shares * all * 4 : 0);
     f.bytes = at;
     return f;

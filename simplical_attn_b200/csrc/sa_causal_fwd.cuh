@@ -1,4 +1,5 @@
-// Causal attention forward on the sm_100a tensor cores (bf16 / fp16, head dim 64 and 128).
+// Causal attention forward on the sm_100a tensor cores (bf16 / fp16; head dims up to 128 that are multiples of 8, in tiles of 64 or
+// 128 columns that the TMA loads fill up with zeros).
 //
 //     S = Q K^T,  P = exp2(S scale log2e - m),  O = sum over key tiles of P V / l,  with the running maximum m and sum l per row.
 //
@@ -495,6 +496,7 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
                     } else {
 #pragma unroll
                         for (int e = 0; e < 32; e += 8) {
+                            if (c0 + e >= p.D) break;
                             uint32_t w[4], lo[4];
 #pragma unroll
                             for (int y = 0; y < 4; ++y) pack_split<F16>(__uint_as_float(x[e + 2 * y]), __uint_as_float(x[e + 2 * y + 1]), w[y], lo[y]);
@@ -514,7 +516,7 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
         }
     }
     if (p.cu_q != nullptr) {
-        zero_outside(o, p.o, p.H, HD, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
+        zero_outside(o, p.o, p.H, p.D, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
         empty_lse_outside(lse, p.H, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
     }
     tc_fence_before();
@@ -584,6 +586,7 @@ __global__ void __launch_bounds__(256) causal_join_kernel(const CParams p, int s
     const int64_t dst = b * p.o.b + (int64_t)n * p.o.n + h * p.o.h + kPer * lane;
 #pragma unroll
     for (int e = 0; e < kPer; e += 2) {
+        if (kPer * lane + e >= p.D) break;
         uint32_t w, low;
         pack_split<F16>(acc[e] * inv, acc[e + 1] * inv, w, low);
         *reinterpret_cast<uint32_t*>(o + dst + e) = w;
@@ -635,24 +638,13 @@ inline FwdPlan plan_fwd(const CParams& c) {
     // Pairs of query tiles that do not fill the multiprocessors are taken apart.
     f.row_tiles = items(2) * c.H > sms ? 2 : 1;
     f.items = items(f.row_tiles);
-    // Shares of the keys, where there are few units: rounds of blocks times the key tiles of the longest unit, with two more
-    // for what a unit costs besides and four for joining, in units of a key tile's time (about 1.5 us).
-    const int64_t units = f.items * c.H;
-    const int tiles = ceil_div(c.max_k, kTile);
-    f.splits = 1;
-    int64_t best = (units + sms - 1) / sms * (tiles + 2);
-    for (int s = 2; s <= 32 && 2 * s <= tiles && units * (s - 1) < 2 * sms; ++s) {
-        const int64_t cost = (units * s + sms - 1) / sms * (ceil_div(tiles, s) + 2) + 4;
-        if (cost < best) {
-            best = cost;
-            f.splits = s;
-        }
-    }
+    // a unit costs about two key tiles' time (1.5 us) besides its own, joining four
+    f.splits = plan_shares(f.items * c.H, ceil_div(c.max_k, kTile), sms, 32, 2, 4);
     size_t at = 0;
     auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };
     f.list = take(c.cu_q != nullptr ? list_bytes(f.items) : 0);
     const size_t rows = (size_t)c.B * c.H * c.Nq;
-    f.part_o = take(f.splits > 1 ? (size_t)f.splits * rows * c.D * 4 : 0);
+    f.part_o = take(f.splits > 1 ? (size_t)f.splits * rows * tile_columns(c.D) * 4 : 0);
     f.part_lse = take(f.splits > 1 ? (size_t)f.splits * rows * 4 : 0);
     f.bytes = at;
     return f;
@@ -664,8 +656,8 @@ int launch_fwd_tc(const CParams& c, const void* q, const void* k, const void* v,
     const FwdPlan f = plan_fwd(c);
     if (f.items * c.H * f.splits > 0x3fffffff) return SA_ERR_UNSUPPORTED;
     CUtensorMap mq, mk, mv;
-    if (!host::make_map(&mq, q, c.B, c.Nq, c.H, HD, c.q, kTile, F16) || !host::make_map(&mk, k, c.B, c.Nk, c.Hkv, HD, c.k, kTile, F16) ||
-        !host::make_map(&mv, v, c.B, c.Nk, c.Hkv, HD, c.v, kTile, F16))
+    if (!host::make_map(&mq, q, c.B, c.Nq, c.H, c.D, c.q, kTile, F16) || !host::make_map(&mk, k, c.B, c.Nk, c.Hkv, c.D, c.k, kTile, F16) ||
+        !host::make_map(&mv, v, c.B, c.Nk, c.Hkv, c.D, c.v, kTile, F16))
         return SA_ERR_BAD_STRIDE;
     FwdParams P{};
     P.c = c;

@@ -61,8 +61,15 @@ PACKED = [
     ([(3, 500), (7, 100), (4, 4), (2, 1), (0, 30)], 4, 1, 64, "fp16"),         # a few tokens: 28 rows
     ([(2, 900), (1, 63)], 5, 5, 128, "fp16"),
     ([(1, 300), (1, 128)], 24, 1, 64, "bf16"),
-    ([(100, 100), (45, 70)], 2, 1, 80, "bf16"),                      # head dims of the general kernels
-    ([(70, 70), (33, 97)], 2, 2, 256, "fp16"),
+    ([(100, 100), (45, 70)], 2, 1, 80, "bf16"),                      # head dims that fill a tile's columns in part
+    ([(140, 140), (3, 200)], 2, 1, 32, "fp16"),
+    ([(20, 150), (1, 77)], 6, 2, 8, "bf16"),
+    ([(130, 257)], 2, 1, 120, "fp16"),
+    ([(70, 70), (33, 97)], 2, 2, 256, "fp16"),                       # ... of the general kernels
+    ([(40, 90), (1, 500)], 2, 1, 100, "bf16"),
+    ([(3, 1500), (40, 700)], 8, 1, 64, "fp32"),                      # few blocks with long walks: shares
+    ([(300, 300)], 8, 1, 200, "fp32"),
+    ([(1, 900), (0, 3)], 2, 2, 33, "fp32"),
     ([(65, 65), (64, 100), (1, 7)], 4, 1, 64, "fp32"),
     ([(90, 33)], 1, 1, 17, "fp32"),
 ]
@@ -440,10 +447,11 @@ def test_entries_validate():
     r = lambda b=0, **kw: lib.sa_causal_resolve(params(**kw), b)
     assert r() == r(1) == r(1, Nq=1) == _abi.SA_ALGO_TCGEN05 and r(Nq=16) == _abi.SA_CAUSAL_FEW_ROWS and r(Nq=17) == _abi.SA_ALGO_TCGEN05
     assert r(Nq=4, algo=_abi.SA_ALGO_TCGEN05) == _abi.SA_ALGO_TCGEN05 and r(sequences=9, max_q=1, max_k=5) == _abi.SA_CAUSAL_FEW_ROWS
-    for general in (dict(D=96), dict(dtype=_abi.SA_F32), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(algo=_abi.SA_ALGO_GENERAL),
+    assert r(D=96) == r(D=8) == r(1, D=40) == _abi.SA_ALGO_TCGEN05
+    for general in (dict(D=100), dict(D=136), dict(dtype=_abi.SA_F32), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(algo=_abi.SA_ALGO_GENERAL),
                     dict(k=_abi.Strides(64 * 512, 512, 132))):
         assert r(**general) == r(1, **general) == _abi.SA_ALGO_GENERAL, general
-    assert r(D=96, algo=_abi.SA_ALGO_TCGEN05) == -4
+    assert r(D=100, algo=_abi.SA_ALGO_TCGEN05) == -4
     assert lib.sa_causal_resolve(params(D=257), 0) == -4 and lib.sa_causal_resolve(params(H=3), 1) == -2
 
 
