@@ -70,14 +70,26 @@ __device__ __forceinline__ void empty_lse_outside(float* lse, int H, int n, cons
 
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Shares that the walks of `units` units, of `steps` steps each at most, are cut into: one where the units fill the
-// multiprocessors, else what makes rounds of units times their steps least.  `around` is what a unit costs besides its steps and
-// `joining` what adding up the shares costs, in steps.
-inline int plan_shares(int64_t units, int steps, int sms, int most, int around, int joining) {
+// Estimated time of `units` walks, of `longest` steps at most and `mean` on average, each cut into `shares`, in steps: walks of
+// different lengths, the longest first, end together; equal ones go by whole rounds over the multiprocessors.
+inline double walk_steps(double units, int longest, double mean, int shares, int sms) {
+    const int share = ceil_div(longest, shares);
+    if (mean < 0.75 * longest) {
+        const double all = units * mean / sms + 0.5;
+        return all > share ? all : share;
+    }
+    return (double)(int64_t)((units * shares + sms - 1) / sms) * share;
+}
+// Steps on average: a causal prompt's queries see half of the keys.
+inline double mean_steps(const CParams& c, int longest) { return c.max_q == c.max_k ? 0.5 * (longest + 1) : longest; }
+
+// Shares of a walk: what makes the estimate least.  `joining` is what adding up shares costs, `each` what every share adds to
+// that, in steps.
+inline int plan_shares(double units, int longest, double mean, int sms, int most, double joining, double each) {
     int shares = 1;
-    int64_t best = (units + sms - 1) / sms * (steps + around);
-    for (int s = 2; s <= most && s <= steps && units * (s - 1) < 2 * sms; ++s) {
-        const int64_t cost = (units * s + sms - 1) / sms * (ceil_div(steps, s) + around) + joining;
+    double best = walk_steps(units, longest, mean, 1, sms);
+    for (int s = 2; s <= most && s <= longest && units * (s - 1) < 2.0 * sms; ++s) {
+        const double cost = walk_steps(units, longest, mean, s, sms) + joining + each * s;
         if (cost < best) {
             best = cost;
             shares = s;

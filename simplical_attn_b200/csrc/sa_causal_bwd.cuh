@@ -174,7 +174,7 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
     uint32_t* tmem_slot = (uint32_t*)(smem + L::kMisc);
     const WaitCtx wctx{base + L::kMisc + 4, P.status, P.wait_limit_ns};
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
     if (tid == 0) {
         auto init = [&](int off, int n, uint32_t count) {
             for (int x = 0; x < n; ++x) mbar_init((uint64_t*)(smem + off) + x, count);
@@ -271,8 +271,11 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
             };
             Ring g;
             uint32_t n = 0, nu = 0;
-            for (Walk w(P, p.Hkv); w.valid(); w.next()) {
-                const ColUnit u = col_unit(P, w);
+            Walk w(P, p.Hkv);
+            make_uniform(w.count);
+            for (; w.valid(); w.next()) {
+                ColUnit u = col_unit(P, w);
+                make_uniform(u.n);
                 if (u.n == 0) continue;
                 mbar_wait<kKvFull>(base, nu & 1, wctx, 3);
                 issue_s(g);
@@ -518,14 +521,23 @@ __device__ __forceinline__ RowUnit row_unit(const BwdParams& P, const Walk& w) {
     return r;
 }
 // The stream of tiles of all units of a block.
+template <bool UNIFORM = false>
 struct RowStream {
     Walk w;
     RowUnit u;
     int t;
-    __device__ __forceinline__ explicit RowStream(const BwdParams& P) : w(P, P.c.H), t(0) { settle(P); }
+    __device__ __forceinline__ explicit RowStream(const BwdParams& P) : w(P, P.c.H), t(0) {
+        if (UNIFORM) make_uniform(w.count);
+        settle(P);
+    }
     __device__ __forceinline__ void settle(const BwdParams& P) {          // at w's unit, or the next that has tiles
         while (w.valid()) {
             u = row_unit(P, w);
+            if (UNIFORM) {
+                make_uniform(u.n);
+                make_uniform(u.t0);
+                make_uniform(u.s.nk);
+            }
             if (u.n > 0) return;
             w.next();
         }
@@ -573,7 +585,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
     uint32_t* tmem_slot = (uint32_t*)(smem + L::kMisc);
     const WaitCtx wctx{base + L::kMisc + 4, P.status, P.wait_limit_ns};
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
     if (tid == 0) {
         auto init = [&](int off, int n, uint32_t count) {
             for (int x = 0; x < n; ++x) mbar_init((uint64_t*)(smem + off) + x, count);
@@ -617,7 +629,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 prefetch_tensormap(&map_do);
                 Ring gk, gv;
                 uint32_t nu = 0;
-                for (RowStream x(P); x.valid(); x.next(P)) {
+                for (RowStream<> x(P); x.valid(); x.next(P)) {
                     const RowUnit& u = x.u;
                     auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head) {
                         mbar_arrive_expect_tx(bar, L::kTileBytes);
@@ -655,7 +667,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 });
             };
             // three positions in the one stream of tiles: where S, dP and dQ are
-            RowStream xs(P), xp(P), xq(P);
+            RowStream<true> xs(P), xp(P), xq(P);
             Ring gs, gp, gq;
             uint32_t ns = 0, np = 0, n = 0, us = 0, up = 0, uq = 0;      // tiles and units so far
             uint32_t s3 = 0, p3 = 0, q3 = 0;                             // tiles modulo 3
@@ -727,7 +739,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
         } else if (warp == 10) {
             // ---------------------------------------------------------------- guard
             Ring g;
-            for (RowStream x(P); x.valid(); x.next(P)) {
+            for (RowStream<> x(P); x.valid(); x.next(P)) {
                 mbar_wait<kKFull>(base + 8 * g.s, g.phase, wctx, 13);
                 const int rows = x.u.s.nk - (x.u.t0 + x.t) * kTile;
                 if (rows < kTile) {
@@ -899,8 +911,13 @@ inline BwdPlan plan_bwd(const CParams& c) {
     f.items_q = packed ? list_capacity(c.Nq, kTile, c.S) : (int64_t)ceil_div(c.Nq, kTile) * c.S;
     f.items_k = packed ? list_capacity(c.Nk, kTile, c.S) : (int64_t)ceil_div(c.Nk, kTile) * c.S;
     const int sms = host::sm_count();
-    f.splits_q = plan_shares(f.items_q * c.H, ceil_div(c.max_k, kTile), sms, 16, 2, 4);
-    f.splits_k = plan_shares(f.items_k * c.Hkv, (int)((int64_t)ceil_div(c.max_q, kTile) * c.G < (1 << 20) ? ceil_div(c.max_q, kTile) * c.G : 1 << 20), sms, 16, 2, 4);
+    // (a step of either kernel takes about 1.3 us, adding shares 3 and the partial rows' way through memory)
+    const double row_us = (double)c.B * tile_columns(c.D) * 8 / 5e6;
+    const int steps_q = ceil_div(c.max_k, kTile);
+    f.splits_q = plan_shares((double)f.items_q * c.H, steps_q, mean_steps(c, steps_q), sms, 16, 2.3, row_us * c.H * c.Nq / 1.3);
+    const int tiles = ceil_div(c.max_q, kTile), steps_k = (int)((int64_t)tiles * c.G < (1 << 20) ? tiles * c.G : 1 << 20);
+    f.splits_k = plan_shares((double)f.items_k * c.Hkv, steps_k, c.max_q == c.max_k ? mean_steps(c, tiles) * c.G : steps_k, sms, 16, 4.6,
+                             2 * row_us * c.Hkv * c.Nk / 1.3);
     size_t at = 0;
     auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };
     f.delta = take((size_t)c.B * c.H * c.Nq * 4);

@@ -147,7 +147,7 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
     int* const bad = (int*)(smem + L::kBad);
     const WaitCtx wctx{base + L::kMisc + 4, P.status, P.wait_limit_ns};
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
     if (tid == 0) {
         auto init = [&](int off, int n, uint32_t count) {
             for (int x = 0; x < n; ++x) mbar_init((uint64_t*)(smem + off) + x, count);
@@ -244,16 +244,25 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
             };
             Ring g;
             FwdWalk w(P);
+            make_uniform(w.count);
+            // (of a unit the issuer only uses its counts of tiles)
+            auto unit = [&] {
+                FwdUnit x = w.unit(P);
+                make_uniform(x.m0);
+                make_uniform(x.m1);
+                x.t0 = uniform(x.first_masked(0));          // the first tile to wait for the guard at
+                return x;
+            };
             FwdUnit u;
             if (w.valid()) {
-                u = w.unit(P);
+                u = unit();
                 first_s(u, g);
             }
             while (w.valid()) {
                 w.next();
                 FwdUnit un = u;
-                if (w.valid()) un = w.unit(P);
-                const int nt = u.tiles(), guarded = u.first_masked(0);
+                if (w.valid()) un = unit();
+                const int nt = u.tiles(), guarded = u.t0;
 #pragma unroll 1
                 for (int t = 0; t < nt; ++t) {
                     g.next<L::kStages>();
@@ -635,11 +644,22 @@ inline FwdPlan plan_fwd(const CParams& c) {
     auto items = [&](int tiles) {
         return c.cu_q != nullptr ? list_capacity(c.Nq, kTile * tiles, c.S) : (int64_t)ceil_div(c.Nq, kTile * tiles) * c.S;
     };
-    // Pairs of query tiles that do not fill the multiprocessors are taken apart.
-    f.row_tiles = items(2) * c.H > sms ? 2 : 1;
+    // A key tile takes a pair of query tiles 1.95 us and a single one 1.75 (D 128; nothing overlaps its softmax); joining shares
+    // takes 3 us and the partial rows' way through memory.
+    const int tiles = ceil_div(c.max_k, kTile);
+    const double mean = mean_steps(c, tiles), each = (double)c.B * c.H * c.Nq * tile_columns(c.D) * 8 / 5e6;
+    double best = 1e30;
+    for (int rt = 2; rt >= 1; --rt) {
+        const double units = (double)items(rt) * c.H, step = rt == 2 ? 1.95 : 1.75;
+        const int s = plan_shares(units, tiles, mean, sms, 32, 3.0 / step, each / step);
+        const double us = walk_steps(units, tiles, mean, s, sms) * step + (s > 1 ? 3.0 + each * s : 0.0);
+        if (us < best) {
+            best = us;
+            f.row_tiles = rt;
+            f.splits = s;
+        }
+    }
     f.items = items(f.row_tiles);
-    // a unit costs about two key tiles' time (1.5 us) besides its own, joining four
-    f.splits = plan_shares(f.items * c.H, ceil_div(c.max_k, kTile), sms, 32, 2, 4);
     size_t at = 0;
     auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };
     f.list = take(c.cu_q != nullptr ? list_bytes(f.items) : 0);

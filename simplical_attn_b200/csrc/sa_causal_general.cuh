@@ -491,9 +491,10 @@ struct GenPlan {
 inline GenPlan plan_general(const CParams& c, bool backward) {
     GenPlan f{};
     const int dp = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256, cols = dp <= 128 ? 64 : 32, sms = host::sm_count();
-    const int64_t steps_k = (int64_t)ceil_div(c.max_q, kGenRows) * c.G;
-    f.shares_q = plan_shares((int64_t)ceil_div(c.max_q, kGenRows) * c.H * c.S, ceil_div(c.max_k, cols), sms, 16, 1, 1);
-    f.shares_k = plan_shares((int64_t)ceil_div(c.max_k, cols) * c.Hkv * c.S, (int)(steps_k < (1 << 20) ? steps_k : 1 << 20), sms, 16, 1, 1);
+    // (a step takes about 4 us, joining 4)
+    const int steps_q = ceil_div(c.max_k, cols), tiles = ceil_div(c.max_q, kGenRows), steps_k = (int)((int64_t)tiles * c.G < (1 << 20) ? tiles * c.G : 1 << 20);
+    f.shares_q = plan_shares((double)tiles * c.H * c.S, steps_q, mean_steps(c, steps_q), sms, 16, 1, 0.05);
+    f.shares_k = plan_shares((double)ceil_div(c.max_k, cols) * c.Hkv * c.S, steps_k, c.max_q == c.max_k ? 0.5 * steps_k : steps_k, sms, 16, 1, 0.05);
     size_t at = 0;
     auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };
     const size_t rows = (size_t)c.B * c.H * c.Nq, keys = (size_t)c.B * c.Hkv * c.Nk;

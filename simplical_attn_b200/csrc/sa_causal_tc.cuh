@@ -9,6 +9,12 @@ namespace causal {
 
 constexpr int kTile = 128;            // rows of a query tile = lanes of tensor memory, and keys of a key tile
 
+// A value that is the same in all lanes, in a form that the compiler knows to be.  The MMA issuer's loops and descriptors then
+// live in uniform registers, which the MMA instructions take their operands from: with tiles and rows that come from memory
+// (or a warp index from threadIdx) every MMA waited for moves between the register files, about 97 cycles to an MMA of 64.
+__device__ __forceinline__ int uniform(int x) { return (int)__reduce_or_sync(0xffffffffu, (unsigned)x); }
+__device__ __forceinline__ void make_uniform(int& x) { x = uniform(x); }
+
 // One entry of a packed batch's list of work: a tile of a sequence.
 struct alignas(32) Item {
     int q0, nq, k0, nk;
