@@ -197,7 +197,7 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
     const uint32_t tm_s = tmem, tm_dp = tmem + kTile, tm_dv = tmem + 2 * kTile, tm_dk = tm_dv + HD;
 
     if (warp >= 8) {
@@ -521,29 +521,19 @@ __device__ __forceinline__ RowUnit row_unit(const BwdParams& P, const Walk& w) {
     return r;
 }
 // The stream of tiles of all units of a block.
-template <bool UNIFORM = false>
 struct RowStream {
     Walk w;
     RowUnit u;
     int t;
-    __device__ __forceinline__ explicit RowStream(const BwdParams& P) : w(P, P.c.H), t(0) {
-        if (UNIFORM) make_uniform(w.count);
-        settle(P);
-    }
+    __device__ __forceinline__ explicit RowStream(const BwdParams& P) : w(P, P.c.H), t(0) { settle(P); }
     __device__ __forceinline__ void settle(const BwdParams& P) {          // at w's unit, or the next that has tiles
         while (w.valid()) {
             u = row_unit(P, w);
-            if (UNIFORM) {
-                make_uniform(u.n);
-                make_uniform(u.t0);
-                make_uniform(u.s.nk);
-            }
             if (u.n > 0) return;
             w.next();
         }
     }
     __device__ __forceinline__ bool valid() const { return w.valid(); }
-    __device__ __forceinline__ bool last() const { return t == u.n - 1; }
     __device__ __forceinline__ void next(const BwdParams& P) {
         if (++t == u.n) {
             t = 0;
@@ -611,7 +601,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
     // Three slots of 128 columns: S of tile n in slot -n mod 3, dP of tile n where S of tile n - 1 was (slot 1 - n mod 3), S of
     // the next tile in the third.
     const uint32_t tm_dq = tmem + 3 * kTile;
@@ -629,7 +619,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 prefetch_tensormap(&map_do);
                 Ring gk, gv;
                 uint32_t nu = 0;
-                for (RowStream<> x(P); x.valid(); x.next(P)) {
+                for (RowStream x(P); x.valid(); x.next(P)) {
                     const RowUnit& u = x.u;
                     auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head) {
                         mbar_arrive_expect_tx(bar, L::kTileBytes);
@@ -666,32 +656,50 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                     mma_ss_lo<off, off>(leader, d, da, db, idesc_s, kk > 0);
                 });
             };
-            // three positions in the one stream of tiles: where S, dP and dQ are
-            RowStream<true> xs(P), xp(P), xq(P);
+            // Three positions in the one stream of tiles: S is up to two tiles ahead of dQ, dP one.  S finds the units and leaves
+            // their numbers of tiles (0: no more) for the others, by unit modulo 4.
+            Walk w(P, p.H);
+            make_uniform(w.count);
+            int n0 = 0, n1 = 0, n2 = 0, n3 = 0;
+            auto tiles_of = [&](uint32_t u) { return u & 2 ? (u & 1 ? n3 : n2) : (u & 1 ? n1 : n0); };
+            uint32_t us = 0, up = 0, uq = 0;                             // units
+            int ts = 0, tp = 0, tq = 0;                                  // tiles of theirs
             Ring gs, gp, gq;
-            uint32_t ns = 0, np = 0, n = 0, us = 0, up = 0, uq = 0;      // tiles and units so far
-            uint32_t s3 = 0, p3 = 0, q3 = 0;                             // tiles modulo 3
+            uint32_t ns = 0, np = 0, n = 0, s3 = 0, p3 = 0, q3 = 0;      // tiles so far, also modulo 3
+            auto find = [&] {
+                int x = 0;
+                for (; w.valid() && x == 0; w.next()) x = uniform(row_unit(P, w).n);
+                if ((us & 3) == 0) n0 = x;
+                else if ((us & 3) == 1) n1 = x;
+                else if ((us & 3) == 2) n2 = x;
+                else n3 = x;
+            };
             auto issue_s = [&] {
-                if (!xs.valid()) return;
-                if (xs.t == 0) mbar_wait<kQFull>(base, us & 1, wctx, 5);
+                const int tiles = tiles_of(us);
+                if (tiles == 0) return;
+                const bool last = ts == tiles - 1;
+                if (ts == 0) mbar_wait<kQFull>(base, us & 1, wctx, 5);
                 mbar_wait<kKFull>(base + 8 * gs.s, gs.phase, wctx, 6);
-                if ((xs.u.t0 + xs.t + 1) * kTile > xs.u.s.nk) mbar_wait<kPassed>(base + 8 * gs.s, gs.phase, wctx, 7);
+                if (last) mbar_wait<kPassed>(base + 8 * gs.s, gs.phase, wctx, 7);      // (keys may end within the last tile)
                 tc_fence_after();
                 scores(tmem + s_slot(s3) * kTile, base + L::kQ, base + L::kKRing + gs.s * L::kTileBytes);
                 if (ns & 1) tc_commit<kSReady + 8>(leader, base);
                 else tc_commit<kSReady>(leader, base);
-                if (xs.last()) {
-                    tc_commit<kQFree>(leader, base);
-                    ++us;
-                }
                 gs.next<L::kKStages>();
                 ++ns;
                 s3 = s3 == 2 ? 0 : s3 + 1;
-                xs.next(P);
+                ++ts;
+                if (last) {
+                    tc_commit<kQFree>(leader, base);
+                    ts = 0;
+                    ++us;
+                    find();
+                }
             };
             auto issue_dp = [&] {
-                if (!xp.valid()) return;
-                if (xp.t == 0) mbar_wait<kDoFull>(base, up & 1, wctx, 8);
+                const int tiles = tiles_of(up);
+                if (tiles == 0) return;
+                if (tp == 0) mbar_wait<kDoFull>(base, up & 1, wctx, 8);
                 mbar_wait<kVFull>(base + 8 * gp.s, gp.phase, wctx, 9);
                 if (np > 0) mbar_wait<kSRead>(base + 8 * ((np - 1) & 1), ((np - 1) >> 1) & 1, wctx, 10);     // S of the tile before is in registers
                 tc_fence_after();
@@ -699,47 +707,50 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 if (np & 1) tc_commit<kDpReady + 8>(leader, base);
                 else tc_commit<kDpReady>(leader, base);
                 tc_commit<kVEmpty>(leader, base + 8 * gp.s);
-                if (xp.last()) {
-                    tc_commit<kDoFree>(leader, base);
-                    ++up;
-                }
                 gp.next<L::kVStages>();
                 ++np;
                 p3 = p3 == 2 ? 0 : p3 + 1;
-                xp.next(P);
+                if (++tp == tiles) {
+                    tc_commit<kDoFree>(leader, base);
+                    tp = 0;
+                    ++up;
+                }
             };
+            find();
             issue_s();
             issue_dp();
             issue_s();
 #pragma unroll 1
-            while (xq.valid()) {
+            for (int tiles = tiles_of(0); tiles > 0;) {
                 // (at the end of a unit dQ goes first: dP of the next unit still waits for its dO)
-                const bool last = xq.last();
+                const bool last = tq == tiles - 1;
                 if (!last) issue_dp();
-                if (xq.t == 0 && uq > 0) mbar_wait<kAccFree>(base, (uq - 1) & 1, wctx, 11);
+                if (tq == 0 && uq > 0) mbar_wait<kAccFree>(base, (uq - 1) & 1, wctx, 11);
                 mbar_wait<kDsReady>(base + 8 * (n & 1), (n >> 1) & 1, wctx, 12);
                 tc_fence_after();
                 const uint32_t a = tmem + dp_slot(q3) * kTile, db = desc_lo(base + L::kKRing + gq.s * L::kTileBytes, L::kSlab);
                 static_for<8>([&](auto kk_c) {
                     constexpr int kk = decltype(kk_c)::value;
-                    mma_ts_lo<(kk >> 2) * 64 + (kk & 3) * 8, kk * (2048 >> 4)>(leader, tm_dq, a, db, idesc_d, xq.t > 0 || kk > 0);
+                    mma_ts_lo<(kk >> 2) * 64 + (kk & 3) * 8, kk * (2048 >> 4)>(leader, tm_dq, a, db, idesc_d, tq > 0 || kk > 0);
                 });
                 tc_commit<kKEmpty>(leader, base + 8 * gq.s);
-                if (last) {
-                    tc_commit<kAccReady>(leader, base);
-                    ++uq;
-                }
                 gq.next<L::kKStages>();
                 ++n;
                 q3 = q3 == 2 ? 0 : q3 + 1;
-                xq.next(P);
-                if (last) issue_dp();
+                ++tq;
+                if (last) {
+                    tc_commit<kAccReady>(leader, base);
+                    tq = 0;
+                    ++uq;
+                    tiles = tiles_of(uq);
+                    issue_dp();
+                }
                 issue_s();
             }
         } else if (warp == 10) {
             // ---------------------------------------------------------------- guard
             Ring g;
-            for (RowStream<> x(P); x.valid(); x.next(P)) {
+            for (RowStream x(P); x.valid(); x.next(P)) {
                 mbar_wait<kKFull>(base + 8 * g.s, g.phase, wctx, 13);
                 const int rows = x.u.s.nk - (x.u.t0 + x.t) * kTile;
                 if (rows < kTile) {

@@ -174,7 +174,7 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
 #define SA_ARRIVE(OFF, BASE)                       \
     do {                                           \
         __syncwarp();                              \
@@ -220,7 +220,7 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
             // ---------------------------------------------------------------- MMA issuer
             const uint32_t leader = elect_one();
             const uint32_t idesc_s = make_idesc(128, kTile, false, false, F16), idesc_o = make_idesc(128, HD, false, true, F16);
-            uint32_t nq[2] = {0, 0}, np[2] = {0, 0};       // units with tiles, tiles so far
+            uint32_t nq0 = 0, nq1 = 0, np0 = 0, np1 = 0;       // per query tile: units with tiles, tiles so far
             auto issue_s = [&](int r, int buf, bool last) {
                 const uint32_t da = desc_lo(base + L::kQ + r * L::kTileBytes, 16), db = desc_lo(base + L::kRing + buf * L::kTileBytes, 16);
                 static_for<HD / 16>([&](auto kk_c) {
@@ -234,12 +234,14 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
             auto first_s = [&](const FwdUnit& u, const Ring& g) {
                 if (u.tiles() == 0) return;
                 mbar_wait<kFull>(base + 8 * g.s, g.phase, wctx, 4);
-                for (int r = 0; r < 2; ++r)
-                    if (u.m(r) > 0) {
-                        mbar_wait<kQFull>(base + 8 * r, nq[r] & 1, wctx, 5);
-                        tc_fence_after();
-                        issue_s(r, g.s, u.m(r) == 1);
-                    }
+                auto one = [&](int r, int m, uint32_t nq) {
+                    if (m == 0) return;
+                    mbar_wait<kQFull>(base + 8 * r, nq & 1, wctx, 5);
+                    tc_fence_after();
+                    issue_s(r, g.s, m == 1);
+                };
+                one(0, u.m0, nq0);
+                one(1, u.m1, nq1);
                 tc_commit<kEmpty>(leader, base + 8 * g.s);
             };
             Ring g;
@@ -272,33 +274,36 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
                     const uint32_t db = desc_lo(base + L::kRing + v.s * L::kTileBytes, L::kSlab);
                     mbar_wait<kFull>(base + 8 * v.s, v.phase, wctx, 6);
                     if (t >= guarded) mbar_wait<kPassed>(base + 8 * v.s, v.phase, wctx, 7);
-#pragma unroll 1
-                    for (int r = 0; r < 2; ++r) {
-                        if (t >= u.m(r)) continue;
+                    // (the query tile as a constant: counters indexed by it would lie in memory)
+                    auto one = [&](auto r_c, int m, uint32_t& nq, uint32_t& np) {
+                        constexpr int r = decltype(r_c)::value;
+                        if (t >= m) return;
                         const uint32_t rb = base + 8 * r, tm_s = tmem + r * kTile, tm_o = tmem + 2 * kTile + r * HD;
-                        if (t == 0 && nq[r] > 0) mbar_wait<kOFree>(rb, (nq[r] - 1) & 1, wctx, 8);
-                        mbar_wait<kPReady>(rb, np[r] & 1, wctx, 9);
+                        if (t == 0 && nq > 0) mbar_wait<kOFree>(rb, (nq - 1) & 1, wctx, 8);
+                        mbar_wait<kPReady>(rb, np & 1, wctx, 9);
                         tc_fence_after();
                         static_for<4>([&](auto kk_c) {
                             constexpr int kk = decltype(kk_c)::value;
                             mma_ts_lo<kk * 8, kk * (2048 >> 4)>(leader, tm_o, tm_s, db, idesc_o, t > 0 || kk > 0);
                         });
-                        mbar_wait<kP2Ready>(rb, np[r] & 1, wctx, 10);
+                        mbar_wait<kP2Ready>(rb, np & 1, wctx, 10);
                         tc_fence_after();
                         static_for<4>([&](auto kk_c) {
                             constexpr int kk = decltype(kk_c)::value + 4;
                             mma_ts_lo<kk * 8, kk * (2048 >> 4)>(leader, tm_o, tm_s, db, idesc_o, true);
                         });
-                        ++np[r];
-                        if (t == u.m(r) - 1) {
+                        ++np;
+                        if (t == m - 1) {
                             tc_commit<kOReady>(leader, rb);
-                            ++nq[r];
+                            ++nq;
                         } else {
                             mbar_wait<kFull>(base + 8 * k.s, k.phase, wctx, 11);
                             tc_fence_after();
-                            issue_s(r, k.s, t + 1 == u.m(r) - 1);
+                            issue_s(r, k.s, t + 1 == m - 1);
                         }
-                    }
+                    };
+                    one(std::integral_constant<int, 0>{}, u.m0, nq0, np0);
+                    one(std::integral_constant<int, 1>{}, u.m1, nq1, np1);
                     tc_commit<kEmpty>(leader, base + 8 * v.s);
                     g.next<L::kStages>();
                     if (t + 1 < nt) tc_commit<kEmpty>(leader, base + 8 * k.s);
