@@ -24,6 +24,9 @@ namespace sa {
 namespace causal {
 
 constexpr int kBwdThreads = 384;
+// Every third pair of the dK / dV kernel's exponentials is taken on the FMA pipes: its two groups are in their exponentials at
+// the same time (861 -> 841 us at B 2 N 8192 H 16/4 D 128).  In the dQ kernel and the forward that was slower.
+constexpr int kFmaCol = 3;
 
 struct BwdParams {
     CParams c;
@@ -376,10 +379,11 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
                     const uint4 x = lds128(stats + c * 4);
                     const float2 y0 = __ffma2_rn(make_float2(pr[c], pr[c + 1]), c2, make_float2(-__uint_as_float(x.x), -__uint_as_float(x.y)));
                     const float2 y1 = __ffma2_rn(make_float2(pr[c + 2], pr[c + 3]), c2, make_float2(-__uint_as_float(x.z), -__uint_as_float(x.w)));
-                    pr[c] = ex2(y0.x);
-                    pr[c + 1] = ex2(y0.y);
-                    pr[c + 2] = ex2(y1.x);
-                    pr[c + 3] = ex2(y1.y);
+                    const float2 e0 = exp2_pair<kFmaCol>(y0, c / 2), e1 = exp2_pair<kFmaCol>(y1, c / 2 + 1);
+                    pr[c] = e0.x;
+                    pr[c + 1] = e0.y;
+                    pr[c + 2] = e1.x;
+                    pr[c + 3] = e1.y;
                 }
                 if (masked) {
 #pragma unroll
@@ -922,12 +926,12 @@ inline BwdPlan plan_bwd(const CParams& c) {
     f.items_q = packed ? list_capacity(c.Nq, kTile, c.S) : (int64_t)ceil_div(c.Nq, kTile) * c.S;
     f.items_k = packed ? list_capacity(c.Nk, kTile, c.S) : (int64_t)ceil_div(c.Nk, kTile) * c.S;
     const int sms = host::sm_count();
-    // (a step of either kernel takes about 1.3 us, adding shares 3 and the partial rows' way through memory)
+    // (a step of either kernel takes about 1.3 us, adding shares 5 for a tensor and the partial rows' way through memory)
     const double row_us = (double)c.B * tile_columns(c.D) * 8 / 5e6;
     const int steps_q = ceil_div(c.max_k, kTile);
-    f.splits_q = plan_shares((double)f.items_q * c.H, steps_q, mean_steps(c, steps_q), sms, 16, 2.3, row_us * c.H * c.Nq / 1.3);
+    f.splits_q = plan_shares((double)f.items_q * c.H, steps_q, mean_steps(c, steps_q), sms, 16, 3.8, row_us * c.H * c.Nq / 1.3);
     const int tiles = ceil_div(c.max_q, kTile), steps_k = (int)((int64_t)tiles * c.G < (1 << 20) ? tiles * c.G : 1 << 20);
-    f.splits_k = plan_shares((double)f.items_k * c.Hkv, steps_k, c.max_q == c.max_k ? mean_steps(c, tiles) * c.G : steps_k, sms, 16, 4.6,
+    f.splits_k = plan_shares((double)f.items_k * c.Hkv, steps_k, c.max_q == c.max_k ? mean_steps(c, tiles) * c.G : steps_k, sms, 16, 7.7,
                              2 * row_us * c.Hkv * c.Nk / 1.3);
     size_t at = 0;
     auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };

@@ -375,6 +375,9 @@ inline FewPlan plan_few(const CParams& c) {
             f.steps = per;
         }
     }
+#ifdef SA_FEW_STEPS
+    f.steps = SA_FEW_STEPS; f.shares = ceil_div(longest, f.steps);
+#endif
     const size_t all = (size_t)c.B * c.H * c.Nq;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };

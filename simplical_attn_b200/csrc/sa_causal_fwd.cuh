@@ -650,14 +650,14 @@ inline FwdPlan plan_fwd(const CParams& c) {
         return c.cu_q != nullptr ? list_capacity(c.Nq, kTile * tiles, c.S) : (int64_t)ceil_div(c.Nq, kTile * tiles) * c.S;
     };
     // A key tile takes a pair of query tiles 1.95 us and a single one 1.75 (D 128; nothing overlaps its softmax); joining shares
-    // takes 3 us and the partial rows' way through memory.
+    // takes 8 us and the partial rows' way through memory.
     const int tiles = ceil_div(c.max_k, kTile);
     const double mean = mean_steps(c, tiles), each = (double)c.B * c.H * c.Nq * tile_columns(c.D) * 8 / 5e6;
     double best = 1e30;
     for (int rt = 2; rt >= 1; --rt) {
         const double units = (double)items(rt) * c.H, step = rt == 2 ? 1.95 : 1.75;
-        const int s = plan_shares(units, tiles, mean, sms, 32, 3.0 / step, each / step);
-        const double us = walk_steps(units, tiles, mean, s, sms) * step + (s > 1 ? 3.0 + each * s : 0.0);
+        const int s = plan_shares(units, tiles, mean, sms, 32, 8.0 / step, each / step);
+        const double us = walk_steps(units, tiles, mean, s, sms) * step + (s > 1 ? 8.0 + each * s : 0.0);
         if (us < best) {
             best = us;
             f.row_tiles = rt;
