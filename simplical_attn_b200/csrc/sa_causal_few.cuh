@@ -3,7 +3,8 @@
 //
 // K and V are read once and little is computed with them: HBM bandwidth bounds it, latency where they are short.  The rows of
 // a block are the queries of all heads that share a KV head (query i, head g of the group: row i G + g), 16 or 32 of them, so a
-// key is read once for the group.  The keys of a sequence are cut into shares, a block each, joined by causal_join_kernel.
+// key is read once for the group.  The keys of a sequence are cut into shares, a block each.  Up to eight shares are a cluster of
+// blocks and join in each other's shared memory; more are joined by causal_join_kernel.
 //
 // The products are 16 x 8 x 16 register MMAs (mma.sync): tcgen05 works on 128 rows, of which these calls would fill 16.  A warp
 // has its own 16 of every 64 keys, copied by its own asynchronous copies into its own part of shared memory, with its own
@@ -17,12 +18,14 @@ namespace causal {
 
 constexpr int kFewThreads = 128;
 constexpr int kFewKeys = 64;              // keys of a step of the block: 16 per warp
+constexpr int kFewCluster = 8;            // blocks of a cluster, at most
 constexpr int kFewRowsMost = 32;          // rows (queries times heads of a group) that these kernels are taken for
 
 struct FewParams {
     CParams c;
     int shares, row_blocks;               // of a sequence's keys, and of its rows
     int steps;                            // steps of a share, at least
+    int cluster;                          // whether the shares of a sequence and head are one cluster
     float* part_o;                        // shares > 1: as in FwdParams
     float* part_lse;
 };
@@ -33,9 +36,9 @@ struct FewLayout {
     static constexpr int kHalf = 16 * HD * 2;                       // 16 rows of K, or of V
     static constexpr int kWarp = kStages * 2 * kHalf;
     static constexpr int kQ = 16 * MT * HD * 2;
-    static constexpr int kStats = 2 * 4 * 16 * MT * 4;              // m, l: [warp][row]
+    static constexpr int kStats = 2 * 5 * 16 * MT * 4;              // m, l: [warp, block][row]
     static constexpr int kBytes = kQ + kStats + 4 * kWarp;
-    static_assert(4 * 16 * MT * HD * 4 <= 4 * kWarp, "the rows of the warps are merged where K and V were");
+    static_assert(5 * 16 * MT * HD * 4 <= 4 * kWarp, "the rows of the warps are merged where K and V were, the block's behind them");
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
@@ -62,15 +65,37 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Whether one of two packed elements is infinite or NaN.
+// Two packed elements, zeros for those that are not finite.
 template <bool F16>
-__device__ __forceinline__ bool not_finite2(uint32_t w) {
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
     constexpr uint32_t kExp = F16 ? 0x7c00u : 0x7f80u;
-    return (~w & kExp) == 0 || (~w & (kExp << 16)) == 0;
+    if ((~w & kExp) == 0) w &= 0xffff0000u;
+    if ((~w & (kExp << 16)) == 0) w &= 0xffffu;
+    return w;
+}
+
+// The blocks of a cluster: all of them here, and another's shared memory.
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t of_rank(uint32_t addr, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
 }
 
 template <int HD, bool F16, int MT>
-__global__ void __launch_bounds__(kFewThreads, MT == 1 ? 2 : 2)
+__global__ void __launch_bounds__(kFewThreads, 2)
 causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ k,
                   const __nv_bfloat16* __restrict__ v, __nv_bfloat16* __restrict__ o, __nv_bfloat16* __restrict__ o_low, float* __restrict__ lse) {
     using L = FewLayout<HD, MT>;
@@ -98,7 +123,7 @@ causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __re
 
     const uint32_t q_st = ptx::smem_u32(smem), w_st = q_st + L::kQ + L::kStats + warp * L::kWarp;
     float* const stat_m = reinterpret_cast<float*>(smem + L::kQ);
-    float* const stat_l = stat_m + 4 * 16 * MT;
+    float* const stat_l = stat_m + 5 * 16 * MT;
     const __nv_bfloat16* const kh = k + s.b * p.k.b + (int64_t)s.k0 * p.k.n + hk * p.k.h;
     const __nv_bfloat16* const vh = v + s.b * p.v.b + (int64_t)s.k0 * p.v.n + hk * p.v.h;
     const float c2 = p.scale * kLog2e;
@@ -236,41 +261,41 @@ causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __re
                 }
                 odd = __any_sync(0xffffffffu, odd);
             }
-            if (!odd) {
-#pragma unroll
-                for (int d = 0; d < HD / 16; ++d) {
-                    uint32_t vb[4];
-                    const int row = ((lane >> 3) & 1) * 8 + (lane & 7), ch = 2 * d + (lane >> 4);
-                    ldm4t(vb, st + L::kHalf + row * HD * 2 + ((ch ^ (row & 7)) << 4));
-#pragma unroll
-                    for (int a = 0; a < MT; ++a) {
-                        mma16816<F16>(acc[a][2 * d], pa[a], vb[0], vb[1]);
-                        mma16816<F16>(acc[a][2 * d + 1], pa[a], vb[2], vb[3]);
-                    }
-                }
-            } else {
-                // key by key, only into rows that see it: a masked zero times it would not be zero
+            if (odd) {
+                // into rows that see them key by key (a masked zero times them would not be zero), then zeros in their place
 #pragma unroll 1
                 for (int j = 0; j < 16; ++j)
 #pragma unroll
-                    for (int a = 0; a < MT; ++a) {
-                        const int from = (lane & ~3) | ((j & 7) >> 1);
-                        const uint32_t w0 = __shfl_sync(0xffffffffu, j < 8 ? pa[a][0] : pa[a][2], from), w1 = __shfl_sync(0xffffffffu, j < 8 ? pa[a][1] : pa[a][3], from);
-                        const float p0 = j & 1 ? E::hi(w0) : E::lo(w0), p1 = j & 1 ? E::hi(w1) : E::lo(w1);
-                        const bool see0 = j0 + j <= last[2 * a], see1 = j0 + j <= last[2 * a + 1];
+                    for (int a = 0; a < MT; ++a)
 #pragma unroll
                         for (int d = 0; d < HD / 8; ++d) {
                             const uint32_t w = ptx::lds32(st + L::kHalf + j * HD * 2 + ((d ^ (j & 7)) << 4) + (lane & 3) * 4);
-                            if (see0) {
-                                acc[a][d][0] = fmaf(p0, E::lo(w), acc[a][d][0]);
-                                acc[a][d][1] = fmaf(p0, E::hi(w), acc[a][d][1]);
-                            }
-                            if (see1) {
-                                acc[a][d][2] = fmaf(p1, E::lo(w), acc[a][d][2]);
-                                acc[a][d][3] = fmaf(p1, E::hi(w), acc[a][d][3]);
+                            if (!not_finite2<F16>(w)) continue;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float x = e & 1 ? E::hi(w) : E::lo(w);
+                                if (!(fabsf(x) < INFINITY) && j0 + j <= last[2 * a + (e >> 1)]) acc[a][d][e] += x;
                             }
                         }
-                    }
+                __syncwarp();
+#pragma unroll 1
+                for (int e = 0; e < 16 * kChunks / 32; ++e) {
+                    const uint32_t at = st + L::kHalf + (lane + 32 * e) * 16;
+                    const uint4 w = ptx::lds128(at);
+                    ptx::sts128(at, make_uint4(finite2<F16>(w.x), finite2<F16>(w.y), finite2<F16>(w.z), finite2<F16>(w.w)));
+                }
+                __syncwarp();
+            }
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) {
+                uint32_t vb[4];
+                const int row = ((lane >> 3) & 1) * 8 + (lane & 7), ch = 2 * d + (lane >> 4);
+                ldm4t(vb, st + L::kHalf + row * HD * 2 + ((ch ^ (row & 7)) << 4));
+#pragma unroll
+                for (int a = 0; a < MT; ++a) {
+                    mma16816<F16>(acc[a][2 * d], pa[a], vb[0], vb[1]);
+                    mma16816<F16>(acc[a][2 * d + 1], pa[a], vb[2], vb[3]);
+                }
             }
         }
         cp_wait<0>();
@@ -298,43 +323,77 @@ causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __re
                 }
         }
         __syncthreads();
+        // row r of the block, columns d .. d + 3, from its rows in `n` places (warps, or blocks of the cluster): the sum relative to
+        // the largest of their maxima, which is left in `top`
+        auto join = [&](int n, auto&& m_of, auto&& l_of, auto&& row_of, float& top, float& sum) {
+            top = -INFINITY;
+            for (int y = 0; y < n; ++y) top = fmaxf(top, m_of(y));
+            const float b = top == -INFINITY ? 0.f : top;
+            float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+            sum = 0.f;
+#pragma unroll 4
+            for (int y = 0; y < n; ++y) {
+                const float w = ptx::ex2(m_of(y) - b);
+                const float4 z = row_of(y);          // (zeros where no key of the row has been seen)
+                sum = fmaf(w, l_of(y), sum);
+                t.x = fmaf(w, z.x, t.x);
+                t.y = fmaf(w, z.y, t.y);
+                t.z = fmaf(w, z.z, t.z);
+                t.w = fmaf(w, z.w, t.w);
+            }
+            return t;
+        };
+        // O and LSE of row rho, columns d .. d + 3, of which t is the sum; `none`: the row has seen no key
+        auto store = [&](int rho, int d, float4 t, float top, float sum, bool none) {
+            const int i = rho / p.G, h = hk * p.G + rho - i * p.G;
+            const int64_t at = ((int64_t)s.b * p.H + h) * p.Nq + s.q0 + i;
+            const float ll = none ? -INFINITY : (top + log2f(sum)) * kLn2, inv = none ? 0.f : 1.f / sum;
+            if (none) t = make_float4(0.f, 0.f, 0.f, 0.f);
+            t = make_float4(t.x * inv, t.y * inv, t.z * inv, t.w * inv);
+            if (P.shares > 1 && !P.cluster) {
+                if (!none) *reinterpret_cast<float4*>(P.part_o + (share * rows_all + at) * HD + d) = t;
+                if (d == 0) P.part_lse[share * rows_all + at] = ll;
+                return;
+            }
+            if (d == 0) lse[at] = ll;
+            if (d >= p.D) return;
+            const int64_t dst = s.b * p.o.b + (int64_t)(s.q0 + i) * p.o.n + h * p.o.h + d;
+            uint2 y, low;
+            pack_split<F16>(t.x, t.y, y.x, low.x);
+            pack_split<F16>(t.z, t.w, y.y, low.y);
+            *reinterpret_cast<uint2*>(o + dst) = y;
+            if (o_low) *reinterpret_cast<uint2*>(o_low + dst) = low;
+        };
+        float* const block = merge + 4 * 16 * MT * HD;              // the block's rows, for the cluster
         for (int c = tid; c < 16 * MT * (HD / 4); c += kFewThreads) {
             const int r = c / (HD / 4), d = c % (HD / 4) * 4, rho = r0 + r;
             if (rho >= R) continue;
-            float top = -INFINITY, w[4], sum = 0.f;
-#pragma unroll
-            for (int y = 0; y < 4; ++y) top = fmaxf(top, stat_m[y * 16 * MT + r]);
-            const float b = top == -INFINITY ? 0.f : top;
-            float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                w[y] = ptx::ex2(stat_m[y * 16 * MT + r] - b);
-                sum += w[y] * stat_l[y * 16 * MT + r];
-                const float4 z = *reinterpret_cast<const float4*>(merge + (y * 16 * MT + r) * HD + (d ^ ((r & 3) << 3)));
-                // (a warp that has seen no key of the row holds zeros)
-                t.x = fmaf(w[y], z.x, t.x);
-                t.y = fmaf(w[y], z.y, t.y);
-                t.z = fmaf(w[y], z.z, t.z);
-                t.w = fmaf(w[y], z.w, t.w);
+            float top, sum;
+            const float4 t = join(4, [&](int y) { return stat_m[y * 16 * MT + r]; }, [&](int y) { return stat_l[y * 16 * MT + r]; },
+                                  [&](int y) { return *reinterpret_cast<const float4*>(merge + (y * 16 * MT + r) * HD + (d ^ ((r & 3) << 3))); }, top, sum);
+            if (P.cluster) {
+                *reinterpret_cast<float4*>(block + r * HD + d) = t;
+                if (d == 0) {
+                    stat_m[4 * 16 * MT + r] = top;
+                    stat_l[4 * 16 * MT + r] = sum;
+                }
+            } else {
+                store(rho, d, t, top, sum, min(rho / p.G + s.off(), c1 - 1) < c0);
             }
-            const int i = rho / p.G, h = hk * p.G + rho - i * p.G;
-            const bool none = min(i + s.off(), c1 - 1) < c0;
-            const float inv = none ? 0.f : 1.f / sum;
-            const int64_t at = ((int64_t)s.b * p.H + h) * p.Nq + s.q0 + i;
-            const float ll = none ? -INFINITY : (top + log2f(sum)) * kLn2;
-            if (none) t = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (P.shares > 1) {
-                if (!none) *reinterpret_cast<float4*>(P.part_o + (share * rows_all + at) * HD + d) = make_float4(t.x * inv, t.y * inv, t.z * inv, t.w * inv);
-                if (d == 0) P.part_lse[share * rows_all + at] = ll;
-            } else if (d < p.D) {
-                const int64_t dst = s.b * p.o.b + (int64_t)(s.q0 + i) * p.o.n + h * p.o.h + d;
-                uint2 y, low;
-                pack_split<F16>(t.x * inv, t.y * inv, y.x, low.x);
-                pack_split<F16>(t.z * inv, t.w * inv, y.y, low.y);
-                *reinterpret_cast<uint2*>(o + dst) = y;
-                if (o_low) *reinterpret_cast<uint2*>(o_low + dst) = low;
-                if (d == 0) lse[at] = ll;
+        }
+        if (P.cluster) {
+            cluster_sync();
+            // (16 MT HD / 4 items dealt out to the blocks)
+            const uint32_t sm = ptx::smem_u32(stat_m + 4 * 16 * MT), sl = ptx::smem_u32(stat_l + 4 * 16 * MT), sb = ptx::smem_u32(block);
+            for (int c = share + P.shares * tid; c < 16 * MT * (HD / 4); c += P.shares * kFewThreads) {
+                const int r = c / (HD / 4), d = c % (HD / 4) * 4, rho = r0 + r;
+                if (rho >= R) continue;
+                float top, sum;
+                const float4 t = join(P.shares, [&](int y) { return ld_cluster(of_rank(sm + r * 4, y)); }, [&](int y) { return ld_cluster(of_rank(sl + r * 4, y)); },
+                                      [&](int y) { return ld_cluster4(of_rank(sb + (r * HD + d) * 4, y)); }, top, sum);
+                store(rho, d, t, top, sum, rho / p.G + s.off() < 0);
             }
+            cluster_sync();                        // (nobody leaves, or writes its rows anew, before all have read them)
         }
         __syncthreads();
     }
@@ -350,7 +409,7 @@ struct FewPlan {
 };
 // Shares of the keys, by an estimate of the time: a round of resident blocks (two to a multiprocessor) costs 1.5 us before its
 // first and after its last step; a step takes 1 us, or what its bytes take of the bandwidth where all of them run; joining
-// takes 3 us and 0.05 for every share.
+// takes 1 us and round in a cluster, else 5 us and 0.05 for every share.
 inline FewPlan plan_few(const CParams& c) {
     FewPlan f{};
     const int rows = (int)((int64_t)c.max_q * c.G < kFewRowsMost ? c.max_q * c.G : kFewRowsMost);
@@ -368,21 +427,19 @@ inline FewPlan plan_few(const CParams& c) {
         double rounds = blocks / slots;
         rounds = rounds <= 1 ? 1 : rounds < 4 ? (double)(int)(rounds + 0.999) : rounds + 0.5;
         const double running = blocks < slots ? blocks : slots, bound = kFewKeys * c.D * 4.0 * running / 6.2e6;
-        const double us = rounds * (1.5 + per * (bound > 1.0 ? bound : 1.0)) + (n > 1 ? 3.0 + 0.05 * n : 0.0);
+        const double us = rounds * (1.5 + per * (bound > 1.0 ? bound : 1.0)) + (n > kFewCluster ? 5.0 + 0.05 * n : n > 1 ? 1.0 * rounds : 0.0);
         if (us < best) {
             best = us;
             f.shares = ceil_div(longest, per);
             f.steps = per;
         }
     }
-#ifdef SA_FEW_STEPS
-    f.steps = SA_FEW_STEPS; f.shares = ceil_div(longest, f.steps);
-#endif
     const size_t all = (size_t)c.B * c.H * c.Nq;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t x = at; at += (n + 255) / 256 * 256; return x; };
-    f.part_o = take(f.shares > 1 ? (size_t)f.shares * all * tile_columns(c.D) * 4 : 0);
-    f.part_lse = take(f.shares > 1 ? (size_t)f.shares * all * 4 : 0);
+    const bool join = f.shares > kFewCluster;
+    f.part_o = take(join ? (size_t)f.shares * all * tile_columns(c.D) * 4 : 0);
+    f.part_lse = take(join ? (size_t)f.shares * all * 4 : 0);
     f.bytes = at;
     return f;
 }
@@ -396,6 +453,7 @@ int launch_few(const CParams& c, const void* q, const void* k, const void* v, vo
     P.c = c;
     P.shares = f.shares;
     P.steps = f.steps;
+    P.cluster = f.shares > 1 && f.shares <= kFewCluster;
     P.row_blocks = f.row_blocks;
     P.part_o = reinterpret_cast<float*>(ws + f.part_o);
     P.part_lse = reinterpret_cast<float*>(ws + f.part_lse);
@@ -403,13 +461,24 @@ int launch_few(const CParams& c, const void* q, const void* k, const void* v, vo
         constexpr int MT = decltype(mt)::value;
         auto kern = causal_few_kernel<HD, F16, MT>;
         if (!allow_dynamic_smem((const void*)kern, FewLayout<HD, MT>::kBytes)) return SA_ERR_LAUNCH;
-        kern<<<(unsigned)grid, kFewThreads, FewLayout<HD, MT>::kBytes, st>>>(P, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v,
-                                                                             (__nv_bfloat16*)o, (__nv_bfloat16*)o_low, lse);
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = (unsigned)f.shares;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = dim3(kFewThreads);
+        cfg.dynamicSmemBytes = FewLayout<HD, MT>::kBytes;
+        cfg.stream = st;
+        cfg.attrs = &attr;
+        cfg.numAttrs = P.cluster ? 1 : 0;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, P, (const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (__nv_bfloat16*)o,
+                                                 (__nv_bfloat16*)o_low, lse);
         host::count_launches(1);
-        return cudaGetLastError() == cudaSuccess ? SA_OK : SA_ERR_LAUNCH;
+        return e == cudaSuccess ? SA_OK : SA_ERR_LAUNCH;
     };
     const int rc = f.mt == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
-    if (rc != SA_OK || f.shares == 1) return rc;
+    if (rc != SA_OK || f.shares == 1 || P.cluster) return rc;
     return launch_join<HD>(c, F16, f.shares, P.part_o, P.part_lse, o, o_low, lse, st);
 }
 

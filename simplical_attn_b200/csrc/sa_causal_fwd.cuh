@@ -10,7 +10,9 @@
 // Warps.  0-3 / 4-7: softmax group of query tile 0 / 1, a row per thread, also writes the rows out.  8: MMA issuer.  9: TMA.
 // 10: V guard (see below).  The query tiles work in opposite phase: while one is in its softmax the tensor cores work for the
 // other.  The issuer's loop runs on over units: S of the next unit's first tile is computed while the rows are written out.
-// Tensor memory: S0 | S1 (128 columns each; P overwrites S as packed 16-bit values) | O0 | O1 (D columns).
+// Tensor memory: S0 | S1 (128 columns each) | O0 | O1 (D columns) | and at D = 64 P0 | P1 (64 columns of packed 16-bit values), which
+// at D = 128 overwrite S.  With columns of its own for P the next S is computed as soon as the softmax has S in registers;
+// at D = 128 it waits for P V.
 //
 // Per pair of query tiles and 128 keys at D = 128 the MMAs take 2048 cycles (128 x 128 x 16 in 64) and so do the exponentials
 // (16 per clock): see the measured figures at the launch.
@@ -48,7 +50,8 @@ struct FwdLayout {
     static constexpr int kSlab = kTile * 128;                    // bytes of a [128 x 64] slab
     static constexpr int kTileBytes = kSlabs * kSlab;
     static constexpr int kStages = HD == 128 ? 5 : 8;            // ring of K and V tiles
-    static constexpr int kMisc = 320;                            // behind the barriers
+    static constexpr bool kOwnP = HD == 64;                      // P beside S in tensor memory, not over it
+    static constexpr int kMisc = 384;                            // behind the barriers
     static constexpr int kBad = 512;                             // guard: [3][HD] first rows that hold +inf, -inf, NaN
     static constexpr int kQ = 2048;
     static constexpr int kRing = kQ + 2 * kTileBytes;
@@ -110,6 +113,12 @@ struct Ring {
     }
 };
 
+// Whether one of two packed elements is infinite or NaN.
+template <bool F16>
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+    constexpr uint32_t kExp = F16 ? 0x7c00u : 0x7f80u;
+    return (~w & kExp) == 0 || (~w & (kExp << 16)) == 0;
+}
 // Two values as packed 16-bit ones, and what that rounding took from them.
 template <bool F16>
 __device__ __forceinline__ void pack_split(float a, float b, uint32_t& w, uint32_t& low) {
@@ -140,7 +149,9 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
     constexpr int kP2Ready = kPReady + 16;            //              second half
     constexpr int kOReady = kP2Ready + 16;            //              O final
     constexpr int kOFree = kOReady + 16;              //              O read out
-    static_assert(kOFree + 16 <= L::kMisc, "room for the barriers");
+    constexpr int kSRead = kOFree + 16;               //              kOwnP: S is in registers
+    constexpr int kPvDone = kSRead + 16;              //              kOwnP: P V of the tile done
+    static_assert(kPvDone + 16 <= L::kMisc, "room for the barriers");
     uint32_t* tmem_slot = (uint32_t*)(smem + L::kMisc);
     volatile int* const bad_unit = (volatile int*)(smem + L::kMisc + 8);      // 1 + index of the unit the noted rows are of
     volatile int* const done = (volatile int*)(smem + L::kMisc + 16);         // [query tile] units whose rows are written out
@@ -161,6 +172,8 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
         init(kP2Ready, 2, 4);
         init(kOReady, 2, 1);
         init(kOFree, 2, 4);
+        init(kSRead, 2, 4);
+        init(kPvDone, 2, 1);
         init(kPassed, L::kStages, 1);
         *(volatile int*)(smem + L::kMisc + 4) = 0;
         *bad_unit = 0;
@@ -234,14 +247,15 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
             auto first_s = [&](const FwdUnit& u, const Ring& g) {
                 if (u.tiles() == 0) return;
                 mbar_wait<kFull>(base + 8 * g.s, g.phase, wctx, 4);
-                auto one = [&](int r, int m, uint32_t nq) {
+                auto one = [&](int r, int m, uint32_t nq, uint32_t np) {
                     if (m == 0) return;
+                    if (L::kOwnP && np > 0) mbar_wait<kSRead>(base + 8 * r, (np - 1) & 1, wctx, 16);
                     mbar_wait<kQFull>(base + 8 * r, nq & 1, wctx, 5);
                     tc_fence_after();
                     issue_s(r, g.s, m == 1);
                 };
-                one(0, u.m0, nq0);
-                one(1, u.m1, nq1);
+                one(0, u.m0, nq0, np0);
+                one(1, u.m1, nq1, np1);
                 tc_commit<kEmpty>(leader, base + 8 * g.s);
             };
             Ring g;
@@ -278,29 +292,36 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
                     auto one = [&](auto r_c, int m, uint32_t& nq, uint32_t& np) {
                         constexpr int r = decltype(r_c)::value;
                         if (t >= m) return;
-                        const uint32_t rb = base + 8 * r, tm_s = tmem + r * kTile, tm_o = tmem + 2 * kTile + r * HD;
+                        const uint32_t rb = base + 8 * r, tm_o = tmem + 2 * kTile + r * HD;
+                        const uint32_t tm_p = L::kOwnP ? tmem + 2 * kTile + 2 * HD + r * (kTile / 2) : tmem + r * kTile;
+                        auto next_s = [&] {
+                            mbar_wait<kFull>(base + 8 * k.s, k.phase, wctx, 11);
+                            if (L::kOwnP) mbar_wait<kSRead>(rb, np & 1, wctx, 16);
+                            tc_fence_after();
+                            issue_s(r, k.s, t + 1 == m - 1);
+                        };
+                        if (L::kOwnP && t + 1 < m) next_s();
                         if (t == 0 && nq > 0) mbar_wait<kOFree>(rb, (nq - 1) & 1, wctx, 8);
                         mbar_wait<kPReady>(rb, np & 1, wctx, 9);
                         tc_fence_after();
                         static_for<4>([&](auto kk_c) {
                             constexpr int kk = decltype(kk_c)::value;
-                            mma_ts_lo<kk * 8, kk * (2048 >> 4)>(leader, tm_o, tm_s, db, idesc_o, t > 0 || kk > 0);
+                            mma_ts_lo<kk * 8, kk * (2048 >> 4)>(leader, tm_o, tm_p, db, idesc_o, t > 0 || kk > 0);
                         });
                         mbar_wait<kP2Ready>(rb, np & 1, wctx, 10);
                         tc_fence_after();
                         static_for<4>([&](auto kk_c) {
                             constexpr int kk = decltype(kk_c)::value + 4;
-                            mma_ts_lo<kk * 8, kk * (2048 >> 4)>(leader, tm_o, tm_s, db, idesc_o, true);
+                            mma_ts_lo<kk * 8, kk * (2048 >> 4)>(leader, tm_o, tm_p, db, idesc_o, true);
                         });
-                        ++np;
+                        if (L::kOwnP) tc_commit<kPvDone>(leader, rb);
                         if (t == m - 1) {
                             tc_commit<kOReady>(leader, rb);
                             ++nq;
-                        } else {
-                            mbar_wait<kFull>(base + 8 * k.s, k.phase, wctx, 11);
-                            tc_fence_after();
-                            issue_s(r, k.s, t + 1 == m - 1);
+                        } else if (!L::kOwnP) {
+                            next_s();
                         }
+                        ++np;
                     };
                     one(std::integral_constant<int, 0>{}, u.m0, nq0, np0);
                     one(std::integral_constant<int, 1>{}, u.m1, nq1, np1);
@@ -357,21 +378,26 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
                     if (t >= guarded) {
                         const uint32_t tile = base + L::kRing + g.s * L::kTileBytes;
                         const int j0 = (u.t0 + t) * kTile, rows = u.s.nk - j0;
-                        constexpr uint32_t kExp = F16 ? 0x7c00u : 0x7f80u;
-                        // a lane takes every 32nd 16-byte chunk; the chunks of a slab's 128-byte row are XOR-ed with row & 7
-#pragma unroll 4
+                        constexpr uint32_t kExp2 = F16 ? 0x7c007c00u : 0x7f807f80u, kOne2 = F16 ? 0x04000400u : 0x00800080u;
+                        // A lane takes every 32nd 16-byte chunk; the chunks of a slab's 128-byte row are XOR-ed with row & 7.  First only
+                        // whether there is anything to note: an exponent of ones carries into its element's sign bit.
+                        uint32_t carry = 0;
+#pragma unroll 8
                         for (int c = lane; c < kTile * HD / 8; c += 32) {
-                            const int sl = c / (kTile * 8), row = c / 8 % kTile;
-                            const uint32_t at = tile + c * 16;
-                            const uint4 x = lds128(at);
-                            const uint32_t word[4] = {x.x, x.y, x.z, x.w};
-                            bool any = false;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) any |= (~word[e] & kExp) == 0 || (~word[e] & (kExp << 16)) == 0;
-                            if (row >= rows) sts128(at, make_uint4(0, 0, 0, 0));
-                            any = any && row < rows;
-                            if (__any_sync(0xffffffffu, any)) note(any, at, x, j0 + row, sl * 64 + (((c & 7) ^ (row & 7)) << 3), units);
+                            const uint4 x = lds128(tile + c * 16);
+                            carry |= ((x.x & kExp2) + kOne2) | ((x.y & kExp2) + kOne2) | ((x.z & kExp2) + kOne2) | ((x.w & kExp2) + kOne2);
                         }
+                        if (__any_sync(0xffffffffu, (carry & 0x80008000u) != 0))
+                            for (int c = lane; c < kTile * HD / 8; c += 32) {
+                                const int sl = c / (kTile * 8), row = c / 8 % kTile;
+                                const uint32_t at = tile + c * 16;
+                                const uint4 x = lds128(at);
+                                const bool any = row < rows && (not_finite2<F16>(x.x) || not_finite2<F16>(x.y) || not_finite2<F16>(x.z) || not_finite2<F16>(x.w));
+                                if (__any_sync(0xffffffffu, any)) note(any, at, x, j0 + row, sl * 64 + (((c & 7) ^ (row & 7)) << 3), units);
+                            }
+                        if (rows < kTile)
+                            for (int c = lane; c < kTile * HD / 8; c += 32)
+                                if (c / 8 % kTile >= rows) sts128(tile + c * 16, make_uint4(0, 0, 0, 0));
                         fence_proxy_async_smem();
                     }
                     SA_ARRIVE(kPassed, base + 8 * g.s);
@@ -386,6 +412,7 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
         const int r = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(row & ~31) << 16;
         const uint32_t s_addr = tmem + r * kTile + lanes, o_addr = tmem + 2 * kTile + r * HD + lanes;
+        const uint32_t p_addr = L::kOwnP ? tmem + 2 * kTile + 2 * HD + r * (kTile / 2) + lanes : s_addr;
         const uint32_t rb = base + 8 * r;
         const float c2 = p.scale * kLog2e;
         uint32_t n = 0, nu = 0, units = 0;
@@ -407,6 +434,10 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
                     ld(2);
                     ld(3);
                     tmem_wait_ld();
+                    if (L::kOwnP) {
+                        tc_fence_before();
+                        SA_ARRIVE(kSRead, rb);
+                    }
                 }
                 if (t >= masked_from) {
                     const int hi = see - t * kTile;
@@ -424,8 +455,12 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
 #pragma unroll
                     for (int y = 0; y < 4; ++y) mx[y] = max3(mx[y], __uint_as_float(v[e + y]), __uint_as_float(v[e + 4 + y]));
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
-                // The running maximum moves only when it has to; then l and O are scaled down.  (O is at rest: this tile's S
-                // was issued behind the last tile's P V.)
+                // The running maximum moves only when it has to; then l and O are scaled down.  (O is at rest, and the columns of P are
+                // free: the last tile's P V is done.  Without kOwnP this tile's S was issued behind it.)
+                if (L::kOwnP && n > 0) {
+                    mbar_wait<kPvDone>(rb, (n - 1) & 1, wctx, 17);
+                    tc_fence_after();
+                }
                 float factor = 1.f;
                 if (top > m + kRescaleLog2 || m == -INFINITY) {
                     if (m > -INFINITY) factor = ex2(m - top);
@@ -456,7 +491,7 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
                         ls[(e >> 1) & 1] = __fadd2_rn(ls[(e >> 1) & 1], pe);
                         pk[e >> 1] = E::pack(pe.x, pe.y);
                     }
-                    tmem_st16(s_addr + c / 2, pk);
+                    tmem_st16(p_addr + c / 2, pk);
                     if (c == kTile / 2 - 32) {
                         tmem_wait_st();
                         tc_fence_before();
