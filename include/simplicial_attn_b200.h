@@ -186,7 +186,7 @@ typedef struct {
     int32_t tensors;             /* 1 to 4 */
     int32_t B, N, D;
     int32_t heads[4];
-    int32_t rotary_dim;          /* even, 2 .. D */
+    int32_t rotary_dim;          /* even, 2 .. D, at most 2048 */
     int32_t interleaved, inverse;
     int32_t dtype;               /* sa_dtype of the tensors */
     int32_t position_bits;       /* 32 or 64 (ignored without positions) */

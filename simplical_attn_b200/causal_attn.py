@@ -175,8 +175,15 @@ def causal_attention(q, k, v, scale: Optional[float] = None, *, cu_q: Optional[t
     device, so a captured call follows what they hold at replay.  `max_q` and `max_k` bound the sequences' lengths; they choose
     kernels and launch shapes, not results.  Rows outside every sequence have O = 0 and zero gradients.
 
-    bf16 and fp16 with head dim 64 or 128 run on tensor cores; other head dims up to 256, fp32 and unaligned strides on the
-    CUDA cores.  The gradients are written without atomics: equal calls give equal bits.  There is no second derivative.
+    bf16 and fp16 with a head dim of at most 128 that is a multiple of 8 run on tensor cores; other head dims up to 256, fp32,
+    unaligned strides and a scale that is not positive on the CUDA cores.  A few queries over many keys (`max_q` times the
+    heads of a K/V head at most 32) have kernels of their own: packed single tokens want `max_q=1`.
+
+    What lies in keys that a query does not see, in rows outside the sequences and in other sequences does not reach a result,
+    NaN and infinities included.  The gradients keep to that between sequences; within one, an element that is not finite may reach
+    gradients across the mask, at most 254 rows away.  They are written without atomics: equal calls give equal bits.  There is no
+    second derivative.  A backward pass is captured into a graph under torch's own condition, that no eager graph of the same leaves is
+    alive.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.dim() and q.shape[-1] else 1.0

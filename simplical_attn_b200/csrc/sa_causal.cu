@@ -20,6 +20,7 @@ int validate(const sa_causal_params* p) {
     if (p->sequences < 0 || p->max_q < 0 || p->max_k < 0 || (p->sequences > 0 && p->B != 1)) return SA_ERR_BAD_SHAPE;
     if (p->dtype < SA_BF16 || p->dtype > SA_F32 || p->D > 256) return SA_ERR_UNSUPPORTED;
     if (p->algo < SA_ALGO_AUTO || p->algo > SA_ALGO_TCGEN05) return SA_ERR_UNSUPPORTED;
+    if ((int64_t)p->B * p->H * p->Nq > 0x7fffffff || (int64_t)p->B * p->Hkv * p->Nk > 0x7fffffff) return SA_ERR_UNSUPPORTED;
     if (p->Nq > (1 << 30) || p->Nk > (1 << 30) || (int64_t)p->H * (p->sequences > 0 ? p->sequences : p->B) > (1 << 30)) return SA_ERR_UNSUPPORTED;
     return SA_OK;
 }
@@ -118,7 +119,7 @@ int sa_causal_resolve(const sa_causal_params* p, int backward) {
 }
 
 int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, const void* v, void* o, void* o_low, float* lse,
-                      const int32_t* cu_q, const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status, void* stream) {
+                      const int32_t* cu_q, const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status, void* stream) try {
     using namespace sa::causal;
     int rc = validate(p);
     if (rc != SA_OK) return rc;
@@ -142,11 +143,13 @@ int sa_causal_forward(const sa_causal_params* p, const void* q, const void* k, c
         if (rc != SA_ERR_BAD_STRIDE || p->algo == SA_ALGO_TCGEN05) return rc;
     }
     return dispatch_general(p->dtype, p->D, [&](auto t, auto d) { return launch_general_fwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, o_low, lse, static_cast<uint8_t*>(workspace), st); });
+} catch (...) {      // (no C++ exception leaves a C entry: out of host memory)
+    return SA_ERR_LAUNCH;
 }
 
 int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, const void* v, const void* o, const void* o_low, const float* lse,
                        const void* d_o, void* dq, void* dk, void* dv, const int32_t* cu_q, const int32_t* cu_k, void* workspace, size_t workspace_bytes, void* status,
-                       void* stream) {
+                       void* stream) try {
     using namespace sa::causal;
     int rc = validate(p);
     if (rc != SA_OK) return rc;
@@ -172,6 +175,8 @@ int sa_causal_backward(const sa_causal_params* p, const void* q, const void* k, 
     return dispatch_general(p->dtype, p->D, [&](auto t, auto d) {
         return launch_general_bwd_d<decltype(t), decltype(d)::value>(c, q, k, v, o, o_low, lse, d_o, dq, dk, dv, static_cast<uint8_t*>(workspace), st);
     });
+} catch (...) {
+    return SA_ERR_LAUNCH;
 }
 
 }  // extern "C"

@@ -157,7 +157,7 @@ def rotary_positions(tensors: Union[torch.Tensor, Sequence[torch.Tensor]], frequ
                      magnitude: float = 1.0, inverse: bool = False, out=None):
     """Rotates one to four tensors [B, N, heads, D] (or packed [T, heads, D]) that share every extent but the heads.
 
-    `frequencies`: float32 or float64 [rotary_dim / 2] radians per position (`rotary_frequencies`).  `positions`: int32 or
+    `frequencies`: float32 or float64 [rotary_dim / 2] radians per position (`rotary_frequencies`), rotary_dim at most 2048.  `positions`: int32 or
     int64, one per row ([N], or [T] of packed rows) or [B, N]; None: rows count from 0.  `offset` is added to either.
     `magnitude` scales the rotated part; `inverse` turns back.  Returns a tensor for a tensor, else a tuple.
 

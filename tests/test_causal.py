@@ -290,7 +290,7 @@ def test_equal_calls_give_equal_bits(algo):
 
 
 @gpu
-@pytest.mark.parametrize("lens", [[(90, 90), (200, 200)], [(1, 700), (1, 1200)]])
+@pytest.mark.parametrize("lens", [[(90, 90), (200, 200)], [(1, 700), (1, 1200)], [(1, 9000), (1, 4000)], [(200, 3000), (30, 700)]])
 def test_captured_call_follows_its_inputs(lens, algo):
     """A captured forward and backward replays on new values and new lengths, and beside another graph."""
     first, (cu_q, cu_k), seqs = make(lens, 4, 2, 64, "bf16", seed=14)
@@ -435,7 +435,7 @@ def test_entries_validate():
         for bad in (dict(B=0), dict(Nq=0), dict(Nk=-1), dict(H=5), dict(Hkv=0), dict(D=0), dict(sequences=-1), dict(max_q=-1),
                     dict(sequences=2, B=2)):
             assert call(params(**bad), some) == 2, bad
-        for bad in (dict(D=257), dict(dtype=3), dict(algo=3), dict(Nk=(1 << 30) + 1)):
+        for bad in (dict(D=257), dict(dtype=3), dict(algo=3), dict(Nk=(1 << 30) + 1), dict(B=1 << 12, Nq=1 << 20)):
             assert call(params(**bad), some) == 4, bad
         assert call(params(sequences=2), some) == 1                       # no starts
         assert call(params(), some, status=nul) == 1

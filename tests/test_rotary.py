@@ -324,7 +324,7 @@ def test_entry_validates():
     for bad in (dict(tensors=0), dict(tensors=5), dict(B=0), dict(N=0), dict(D=0), dict(rotary_dim=0), dict(rotary_dim=63), dict(rotary_dim=66),
                 dict(heads=[4, 0, 0, 0])):
         assert call(**bad) == 2, bad
-    for bad in (dict(dtype=3), dict(frequency_bits=16), dict(pos=4096, position_bits=16), dict(B=1 << 16, N=1 << 16)):
+    for bad in (dict(dtype=3), dict(frequency_bits=16), dict(pos=4096, position_bits=16), dict(B=1 << 16, N=1 << 16), dict(D=4096, rotary_dim=2050)):
         assert call(**bad) == 4, bad
 
 
