@@ -47,14 +47,16 @@ __global__ void __launch_bounds__(256) causal_delta16_kernel(const CParams p, co
     using E = ptx::El<F16>;
     constexpr int kLanes = HD / 8;
     const int lane = threadIdx.x % kLanes;
-    const int64_t w = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+    // (rows fit 31 bits; 64-bit divisions took most of this kernel's time)
+    const unsigned w = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
     float sum = 0.f;
     int h = 0, i = 0, b = 0;
-    const bool in = w < (int64_t)p.B * p.Nq * p.H;
+    const bool in = w < (unsigned)(p.B * p.Nq * p.H);
     if (in) {
-        h = (int)(w % p.H);
-        i = (int)(w / p.H % p.Nq);
-        b = (int)(w / p.H / p.Nq);
+        const unsigned bi = w / (unsigned)p.H;
+        h = (int)(w - bi * (unsigned)p.H);
+        b = (int)(bi / (unsigned)p.Nq);
+        i = (int)(bi - (unsigned)b * (unsigned)p.Nq);
         const int64_t at = b * p.o.b + i * p.o.n + h * p.o.h + 8 * lane;
         const uint4 none = make_uint4(0, 0, 0, 0);
         const bool col = 8 * lane < p.D;
@@ -887,10 +889,13 @@ template <int HD, bool F16>
 __global__ void __launch_bounds__(256) causal_add_kernel(const float* __restrict__ part, __nv_bfloat16* __restrict__ out, sa_strides so, int splits, int B,
                                                         int heads, int n, int D, const int* cu, int S) {
     using E = ptx::El<F16>;
-    const int64_t rows = (int64_t)B * heads * n, idx = (int64_t)blockIdx.x * 256 + threadIdx.x, at = idx / (HD / 4);
-    const int c = (int)(idx % (HD / 4)) * 4;
+    constexpr int kRows = 256 / (HD / 4);          // of a block
+    const int64_t rows = (int64_t)B * heads * n;
+    const unsigned at = blockIdx.x * kRows + threadIdx.x / (HD / 4);
+    const int c = (int)(threadIdx.x % (HD / 4)) * 4;
     if (at >= rows || c >= D) return;
-    const int i = (int)(at % n), h = (int)(at / n % heads), b = (int)(at / n / heads);
+    const unsigned bh = at / (unsigned)n;
+    const int i = (int)(at - bh * (unsigned)n), h = (int)(bh % (unsigned)heads), b = (int)(bh / (unsigned)heads);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (cu == nullptr || (i >= cu[0] && i < cu[S])) {         // (rows outside every sequence: zeros)
 #pragma unroll 4

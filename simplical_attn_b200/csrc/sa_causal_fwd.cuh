@@ -590,7 +590,8 @@ __global__ void __launch_bounds__(256) causal_join_kernel(const CParams p, int s
     ptx::griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, member = warp % team;
     const int64_t rows = (int64_t)p.B * p.H * p.Nq, at = (int64_t)blockIdx.x * (8 / team) + warp / team;
-    const int n = (int)(at % p.Nq), h = (int)(at / p.Nq % p.H), b = (int)(at / p.Nq / p.H);
+    const unsigned bh = (unsigned)at / (unsigned)p.Nq;          // (rows fit 31 bits)
+    const int n = (int)((unsigned)at - bh * (unsigned)p.Nq), h = (int)(bh % (unsigned)p.H), b = (int)(bh / (unsigned)p.H);
     // (rows outside the sequences are written where the shares are)
     const bool in = at < rows && (p.cu_q == nullptr || (n >= p.cu_q[0] && n < p.cu_q[p.S]));
     float top = -INFINITY, sum = 0.f, acc[kPer];
