@@ -8,14 +8,19 @@
 // That computes S and dO V^T twice: 7 products of 128 x 128 x D per pair of tiles instead of 5.  In exchange nothing is
 // written that is not a result, and equal calls give equal bits.
 //
-// Both are persistent, with warps 0-3 and 4-7 (compute) each at one half of a tile's columns and a row of tensor memory per
-// thread, warp 8 issuing MMAs, warp 9 TMA loads, warp 10 guarding: it zeroes the rows behind a sequence's end in tiles that
+// Both are persistent, with groups of four warps (compute) each at a share of a tile's columns and a row of tensor memory per
+// thread -- two groups (dK, dV) or four (dQ: 700 -> 580 us at D = 64 of the size below; for dK, dV no difference) --, then a warp
+// issuing MMAs, one TMA loads, one guarding: it zeroes the rows behind a sequence's end in tiles that
 // the MMAs sum over (they belong to the next sequence, and a masked zero times its NaN would not be zero), and in the dK / dV
 // kernel loads LSE and Delta of the query tile.  P and dS go from registers to tensor memory and from there into the MMA as
-// the A operand; a half tile's packed values lie in the columns of that half's scores.
+// the A operand; a group's packed values lie in the columns of its scores.
 //
 // The streams of tiles run on over units: while the rows of a finished unit are written out, the next one's scores are
-// computed.  MMA cycles per pair of tiles at D = 128: 2048 (dK, dV), 1536 (dQ); exponentials take 1024 of either.
+// computed.  MMA cycles per pair of tiles at D = 128: 2048 (dK, dV), 1536 (dQ); exponentials take 1024 of either, and operand reads
+// and TMA writes of shared memory 2290 and 1792.
+//
+// Measured, bf16 B 2 N 8192 H 16/4: D 128 dK, dV 821 us (1340 TFLOP/s of its four products), dQ 644 us (1280 of three); D 64 745 and
+// 565 us.  Steps take about 2890 and 2310 cycles at D 128.
 #pragma once
 
 #include "sa_causal_fwd.cuh"
@@ -23,7 +28,15 @@
 namespace sa {
 namespace causal {
 
-constexpr int kBwdThreads = 384;
+constexpr int kColThreads = 384;                     // dK, dV: two compute groups
+constexpr int kRowThreads = 640;                     // dQ: four
+constexpr int kRowGroups = 4;
+constexpr int kRowCols = kTile / kRowGroups;         // columns of a tile that a group of the dQ kernel has
+constexpr int kRowWarps = 4 * kRowGroups;            // its compute warps; behind them MMA issuer, TMA, guard
+constexpr int kRowRegsCompute = 104, kRowRegsRest = 64;
+static_assert(kRowGroups * kRowRegsCompute + kRowRegsRest <= 5 * 96, "register pool of the block (640 x 96 at launch)");
+// A operand columns of the k-th step of 16: a group's packed values lie in the first half of its columns.
+constexpr int packed_column(int k, int cols) { return k / (cols / 16) * cols + k % (cols / 16) * 8; }
 // Every third pair of the dK / dV kernel's exponentials is taken on the FMA pipes: its two groups are in their exponentials at
 // the same time (861 -> 841 us at B 2 N 8192 H 16/4 D 128).  In the dQ kernel and the forward that was slower.
 constexpr int kFmaCol = 3;
@@ -152,7 +165,7 @@ struct ColStep {
 };
 
 template <int HD, bool F16>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(kColThreads, 1)
 causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, __nv_bfloat16* __restrict__ dk,
                      __nv_bfloat16* __restrict__ dv) {
@@ -258,7 +271,7 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
                 const uint32_t db = desc_lo(b_tile, L::kSlab);
                 static_for<8>([&](auto kk_c) {
                     constexpr int kk = decltype(kk_c)::value;
-                    mma_ts_lo<(kk >> 2) * 64 + (kk & 3) * 8, kk * (2048 >> 4)>(leader, d, a, db, idesc_d, !first || kk > 0);
+                    mma_ts_lo<packed_column(kk, kTile / 2), kk * (2048 >> 4)>(leader, d, a, db, idesc_d, !first || kk > 0);
                 });
             };
             auto stage = [&](const Ring& g) { return base + L::kRing + g.s * 2 * L::kTileBytes; };
@@ -550,7 +563,7 @@ struct RowStream {
 };
 
 template <int HD, bool F16>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(kRowThreads, 1)
 causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, __nv_bfloat16* __restrict__ dq) {
     using L = RowLayout<HD>;
@@ -592,15 +605,15 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
         init(kVFull, 2 * L::kVStages, 1);
         init(kQFull, 4, 1);
         init(kSReady, 2, 1);
-        init(kSRead, 2, 8);
+        init(kSRead, 2, kRowWarps);
         init(kDpReady, 2, 1);
-        init(kDsReady, 2, 8);
+        init(kDsReady, 2, kRowWarps);
         init(kAccReady, 1, 1);
-        init(kAccFree, 1, 8);
+        init(kAccFree, 1, kRowWarps);
         *(volatile int*)(smem + L::kMisc + 4) = 0;
         fence_mbar_init();
     }
-    if (warp == 8) {
+    if (warp == kRowWarps) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -614,9 +627,9 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
     auto s_slot = [](uint32_t m3) { return m3 == 0 ? 0u : 3u - m3; };
     auto dp_slot = [](uint32_t m3) { return m3 == 0 ? 1u : m3 == 1 ? 0u : 2u; };
 
-    if (warp >= 8) {
-        reg_dealloc<kFwdRegsRest>();
-        if (warp == 9) {
+    if (warp >= kRowWarps) {
+        reg_dealloc<kRowRegsRest>();
+        if (warp == kRowWarps + 1) {
             // ---------------------------------------------------------------- TMA
             if (lane == 0) {
                 prefetch_tensormap(&map_q);
@@ -651,7 +664,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 }
             }
             __syncwarp();
-        } else if (warp == 8) {
+        } else if (warp == kRowWarps) {
             // ---------------------------------------------------------------- MMA issuer:  dP(n + 1), dQ(n), S(n + 2)
             const uint32_t leader = elect_one();
             const uint32_t idesc_s = make_idesc(128, kTile, false, false, F16), idesc_d = make_idesc(128, HD, false, true, F16);
@@ -737,7 +750,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 const uint32_t a = tmem + dp_slot(q3) * kTile, db = desc_lo(base + L::kKRing + gq.s * L::kTileBytes, L::kSlab);
                 static_for<8>([&](auto kk_c) {
                     constexpr int kk = decltype(kk_c)::value;
-                    mma_ts_lo<(kk >> 2) * 64 + (kk & 3) * 8, kk * (2048 >> 4)>(leader, tm_dq, a, db, idesc_d, tq > 0 || kk > 0);
+                    mma_ts_lo<packed_column(kk, kRowCols), kk * (2048 >> 4)>(leader, tm_dq, a, db, idesc_d, tq > 0 || kk > 0);
                 });
                 tc_commit<kKEmpty>(leader, base + 8 * gq.s);
                 gq.next<L::kKStages>();
@@ -753,7 +766,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 }
                 issue_s();
             }
-        } else if (warp == 10) {
+        } else if (warp == kRowWarps + 2) {
             // ---------------------------------------------------------------- guard
             Ring g;
             for (RowStream x(P); x.valid(); x.next(P)) {
@@ -769,8 +782,8 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
             }
         }
     } else {
-        // -------------------------------------------------------------------- compute: a query per thread, 64 keys per group
-        reg_alloc<kFwdRegsSoftmax>();
+        // -------------------------------------------------------------------- compute: a query per thread, 32 keys per group
+        reg_alloc<kRowRegsCompute>();
         const int grp = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(row & ~31) << 16;
         const float2 c2 = make_float2(p.scale * kLog2e, p.scale * kLog2e), sc = make_float2(p.scale, p.scale);
@@ -789,78 +802,74 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
             const int masked_from = u.first_masked();
 #pragma unroll 1
             for (int t = 0; t < u.n; ++t, ++n) {
-                const uint32_t s_addr = tmem + s_slot(n3) * kTile + lanes + 64 * grp, dp_addr = tmem + dp_slot(n3) * kTile + lanes + 64 * grp;
+                const uint32_t s_addr = tmem + s_slot(n3) * kTile + lanes + kRowCols * grp, dp_addr = tmem + dp_slot(n3) * kTile + lanes + kRowCols * grp;
                 n3 = n3 == 2 ? 0 : n3 + 1;
                 mbar_wait<kSReady>(base + 8 * (n & 1), (n >> 1) & 1, wctx, 14);
                 tc_fence_after();
-                float pr[64];
+                float pr[kRowCols];
                 tmem_ld32(s_addr, reinterpret_cast<uint32_t(&)[32]>(pr[0]));
-                tmem_ld32(s_addr + 32, reinterpret_cast<uint32_t(&)[32]>(pr[32]));
                 tmem_wait_ld();
                 tc_fence_before();
                 SA_ARRIVE(kSRead, base + 8 * (n & 1));
                 const bool masked = t >= masked_from;
-                uint32_t seen[2] = {~0u, ~0u};
+                uint32_t seen = ~0u;
                 if (masked) {
-                    const int hi = i + u.s.off() - (u.t0 + t) * kTile - 64 * grp;        // columns up to this one
-                    seen[0] = hi >= 31 ? ~0u : hi < 0 ? 0u : ~0u >> (31 - hi);
-                    seen[1] = hi >= 63 ? ~0u : hi < 32 ? 0u : ~0u >> (63 - hi);
+                    const int hi = i + u.s.off() - (u.t0 + t) * kTile - kRowCols * grp;        // columns up to this one
+                    seen = hi >= 31 ? ~0u : hi < 0 ? 0u : ~0u >> (31 - hi);
                 }
 #pragma unroll
-                for (int c = 0; c < 64; c += 2) {
+                for (int c = 0; c < kRowCols; c += 2) {
                     const float2 y = __ffma2_rn(make_float2(pr[c], pr[c + 1]), c2, nls);
                     pr[c] = ex2(y.x);
                     pr[c + 1] = ex2(y.y);
                 }
                 mbar_wait<kDpReady>(base + 8 * (n & 1), (n >> 1) & 1, wctx, 15);
                 tc_fence_after();
+                uint32_t v[kRowCols], pk[kRowCols / 2];
+                tmem_ld32(dp_addr, v);
+                tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 64; c += 32) {
-                    uint32_t v[32], pk[16];
-                    tmem_ld32(dp_addr + c, v);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float2 y = __ffma2_rn(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc, ndl);
-                        y = __fmul2_rn(y, make_float2(pr[c + e], pr[c + e + 1]));
-                        if (masked) {
-                            y.x = (seen[c >> 5] >> e) & 1 ? y.x : 0.f;
-                            y.y = (seen[c >> 5] >> e) & 2 ? y.y : 0.f;
-                        }
-                        pk[e >> 1] = E::pack(y.x, y.y);
+                for (int e = 0; e < kRowCols; e += 2) {
+                    float2 y = __ffma2_rn(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc, ndl);
+                    y = __fmul2_rn(y, make_float2(pr[e], pr[e + 1]));
+                    if (masked) {
+                        y.x = (seen >> e) & 1 ? y.x : 0.f;
+                        y.y = (seen >> e) & 2 ? y.y : 0.f;
                     }
-                    tmem_st16(dp_addr + c / 2, pk);
+                    pk[e >> 1] = E::pack(y.x, y.y);
                 }
+                tmem_st16(dp_addr, pk);
                 tmem_wait_st();
                 tc_fence_before();
                 SA_ARRIVE(kDsReady, base + 8 * (n & 1));
             }
-            // ---- each group writes half of the columns
+            // ---- each group writes a quarter of the columns
             if (u.n > 0) {
                 mbar_wait<kAccReady>(base, nu & 1, wctx, 16);
                 tc_fence_after();
                 ++nu;
             }
-            const int col = grp * (HD / 2);
+            constexpr int kOut = HD / kRowGroups;
+            const int col = grp * kOut;
             __nv_bfloat16* const dst = dq + u.s.b * p.dq.b + (int64_t)(u.s.q0 + i) * p.dq.n + u.h * p.dq.h + col;
             float* const part = P.part0 + (int64_t)u.split * p.B * p.H * p.Nq * HD + at * HD + col;
 #pragma unroll
-            for (int c0 = 0; c0 < HD / 2; c0 += 32) {
-                uint32_t x[32];
+            for (int c0 = 0; c0 < kOut; c0 += 16) {
+                uint32_t x[16];
                 if (u.n > 0) {
-                    tmem_ld32(tm_dq + lanes + col + c0, x);
+                    tmem_ld16(tm_dq + lanes + col + c0, x);
                     tmem_wait_ld();
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] = 0u;
+                    for (int e = 0; e < 16; ++e) x[e] = 0u;
                 }
                 if (!mine) continue;
                 if (P.splits > 1) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + c0 + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                    for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(part + c0 + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8)
+                    for (int e = 0; e < 16; e += 8)
                         if (col + c0 + e < p.D)
                             *reinterpret_cast<uint4*>(dst + c0 + e) =
                                 make_uint4(E::pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), E::pack(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])),
@@ -876,7 +885,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
     if (p.cu_q != nullptr && P.splits == 1) zero_outside(dq, p.dq, p.H, p.D, p.Nq, p.cu_q, p.S, blockIdx.x, gridDim.x);
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kRowWarps) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -996,7 +1005,7 @@ int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v,
         P.part0 = reinterpret_cast<float*>(ws + f.part_k);
         P.part1 = reinterpret_cast<float*>(ws + f.part_v);
         const int64_t units = f.items_k * c.Hkv * f.splits_k;
-        causal_dkv_tc_kernel<HD, F16><<<(unsigned)(units < sms ? units : sms), kBwdThreads, ColLayout<HD>::kBytes, st>>>(
+        causal_dkv_tc_kernel<HD, F16><<<(unsigned)(units < sms ? units : sms), kColThreads, ColLayout<HD>::kBytes, st>>>(
             P, mq, mk, mv, mo, (__nv_bfloat16*)dk, (__nv_bfloat16*)dv);
         host::count_launches(1);
         if (f.splits_k > 1) {
@@ -1011,7 +1020,7 @@ int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v,
         P.splits = f.splits_q;
         P.part0 = reinterpret_cast<float*>(ws + f.part_q);
         const int64_t units = f.items_q * c.H * f.splits_q;
-        causal_dq_tc_kernel<HD, F16><<<(unsigned)(units < sms ? units : sms), kBwdThreads, RowLayout<HD>::kBytes, st>>>(P, mq, mk, mv, mo, (__nv_bfloat16*)dq);
+        causal_dq_tc_kernel<HD, F16><<<(unsigned)(units < sms ? units : sms), kRowThreads, RowLayout<HD>::kBytes, st>>>(P, mq, mk, mv, mo, (__nv_bfloat16*)dq);
         host::count_launches(1);
         if (f.splits_q > 1) rc = launch_add<HD>(F16, P.part0, dq, c.dq, f.splits_q, c.B, c.H, c.Nq, c.D, c.cu_q, c.S, st);
     }

@@ -9,6 +9,10 @@
 // The products are 16 x 8 x 16 register MMAs (mma.sync): tcgen05 works on 128 rows, of which these calls would fill 16.  A warp
 // has its own 16 of every 64 keys, copied by its own asynchronous copies into its own part of shared memory, with its own
 // running maximum, sum and rows of O: warps wait for nobody until they are merged at the end.
+//
+// Measured: 64 sequences of one token over 4096 keys, H 32/8, D 128: 164 us, 6.5 TB/s; 16 over 8192, H 32/2: 28.5 us in a graph;
+// one over 2001, H 16/4, D 64: 6.6 us in a graph.  Sequences of different lengths leave the last round of blocks part empty: 16 of
+// 2 to 16 K keys 42 us, 3.4 TB/s.
 #pragma once
 
 #include "sa_causal_fwd.cuh"

@@ -32,7 +32,7 @@ __device__ __forceinline__ float2 exp2_pair(float2 x, int i) {
 
 // A value that is the same in all lanes, in a form that the compiler knows to be.  The MMA issuer's loops and descriptors then
 // live in uniform registers, which the MMA instructions take their operands from: with tiles and rows that come from memory
-// (or a warp index from threadIdx) every MMA waited for moves between the register files, about 97 cycles to an MMA of 64.
+// (or a warp index from threadIdx) every MMA waited for moves between the register files (dQ kernel at D 128: 855 -> 695 us).
 __device__ __forceinline__ int uniform(int x) { return (int)__reduce_or_sync(0xffffffffu, (unsigned)x); }
 __device__ __forceinline__ void make_uniform(int& x) { x = uniform(x); }
 
@@ -91,7 +91,7 @@ __host__ __device__ inline int first_query(int j0, int nq, int nk) {       // a 
 }
 
 // The lists of a packed batch, a block for each: tiles of `rows[list]` queries (keys where by_key[list]), sorted by cost in one
-// counting pass.  Items of equal cost come in any order: it decides where they run, not what they compute.
+// counting pass (4.4 us for 9 sequences of 11 K rows).  Items of equal cost come in any order: it decides where they run, not what they compute.
 struct PlanParams {
     ListHead* list[2];
     int rows[2], by_key[2];
