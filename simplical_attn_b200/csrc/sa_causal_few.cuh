@@ -424,9 +424,11 @@ inline FewPlan plan_few(const CParams& c) {
     const double heads = (double)c.Hkv * f.row_blocks, slots = 2.0 * host::sm_count();
     const double total = packed ? (double)c.Nk / kFewKeys + 0.5 * c.S : (double)longest * c.S;      // steps of a head
     double best = 1e30;
-    for (int n = 1; n <= 128 && n <= longest; ++n) {
+    // (a dozen of counts up to 16, then steps of an eighth: this runs on the host before every call)
+    for (int n = 1, last = 0; n <= 128 && n <= longest; n += n < 16 ? 1 : n / 8) {
         const int per = ceil_div(longest, n);
-        if (n > 1 && per == ceil_div(longest, n - 1)) continue;
+        if (per == last) continue;
+        last = per;
         const double blocks = heads * (packed ? (total / per < c.S ? c.S : total / per + 0.5 * c.S) : (double)ceil_div(longest, per) * c.S);
         double rounds = blocks / slots;
         rounds = rounds <= 1 ? 1 : rounds < 4 ? (double)(int)(rounds + 0.999) : rounds + 0.5;

@@ -134,7 +134,7 @@ class RotaryPositionsFunction(torch.autograd.Function):
         of = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[6 + i]]
         out = [None] * len(grads)
         if of:
-            for i, g in zip(of, _rotate([grads[i] for i in of], frequencies, positions, offset, interleaved, magnitude, not inverse)):
+            for i, g in zip(of, _rotate(tuple(grads[i] for i in of), frequencies, positions, offset, interleaved, magnitude, not inverse)):
                 out[i] = g
         return (None,) * 6 + tuple(out)
 
@@ -142,9 +142,11 @@ class RotaryPositionsFunction(torch.autograd.Function):
 def _rotate(xs, frequencies, positions, offset, interleaved, magnitude, inverse, out=None):
     native = _native()
     if native is not None:
-        r = native.rotary(tuple(xs), out, frequencies, positions, offset, interleaved, magnitude, inverse)
+        r = native.rotary(xs, out, frequencies, positions, offset, interleaved, magnitude, inverse)
         if r is not None:
             return r
+    if not all(isinstance(t, torch.Tensor) for t in xs):
+        raise TypeError("rotary_positions takes a tensor or a sequence of one to four tensors")
     if torch.is_grad_enabled() and frequencies.requires_grad:
         raise ValueError("there is no gradient for the frequencies")
     if out is not None:
@@ -166,12 +168,12 @@ def rotary_positions(tensors: Union[torch.Tensor, Sequence[torch.Tensor]], frequ
     """
     one = isinstance(tensors, torch.Tensor)
     xs = (tensors,) if one else tuple(tensors)
-    if not xs or not all(isinstance(t, torch.Tensor) for t in xs):
+    if not xs:
         raise TypeError("rotary_positions takes a tensor or a sequence of one to four tensors")
     if out is not None:
         out = (out,) if isinstance(out, torch.Tensor) else tuple(out)
-    r = _rotate(xs, frequencies, positions, int(offset), bool(interleaved), float(magnitude), bool(inverse), out)
-    return r[0] if one else tuple(r)
+    r = _rotate(xs, frequencies, positions, offset, interleaved, magnitude, inverse, out)
+    return r[0] if one else r
 
 
 class RotaryPositions(torch.nn.Module):
