@@ -340,6 +340,24 @@ def test_two_streams_at_once(algo):
 
 
 @gpu
+@pytest.mark.parametrize("direction,label", [(2, "sa_causal_forward"), (3, "sa_causal_backward")])
+def test_report_of_an_earlier_call_is_raised_once(direction, label):
+    """What a kernel that gave up on a wait leaves in the pinned word of its kind of call (here: the library's self-test) is raised by
+    the next call."""
+    lib = _abi.load()
+    word = ctypes.c_void_p(_abi.binding().status_word(torch.cuda.current_device(), direction))
+    q = torch.randn(1, 70, 2, 64, device="cuda", dtype=torch.bfloat16)
+    o = sab.causal_attention(q, q, q)
+    for ask in (lambda: sab.causal_attention(q, q, q), sab.check_device_status):
+        assert lib.sa_selftest_wait_timeout(word, 2_000_000, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == _abi.SA_OK
+        torch.cuda.synchronize()
+        with pytest.raises(_abi.SimplicialAttnError, match=label):
+            ask()
+        ask()
+    assert torch.equal(sab.causal_attention(q, q, q), o)
+
+
+@gpu
 def test_nothing_to_do():
     for q_rows, k_rows in ((0, 0), (0, 5), (5, 0)):
         q = torch.randn(2, q_rows, 4, 64, device="cuda", dtype=torch.bfloat16)
