@@ -108,7 +108,7 @@ size_t sa_causal_backward_workspace_size(const sa_causal_params* p) {
     const int algo = resolve(p, true);
     if (algo < 0) return 0;
     const CParams c = planned(p);
-    const size_t general = plan_general(c, true).bytes, own = algo == SA_ALGO_TCGEN05 ? plan_bwd(c).bytes : 0;
+    const size_t general = plan_general(c, true).bytes, own = algo == SA_ALGO_TCGEN05 ? plan_bwd(c, p->dtype == SA_F16).bytes : 0;
     return general > own ? general : own;
 }
 

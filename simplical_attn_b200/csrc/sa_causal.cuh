@@ -27,6 +27,7 @@ inline int tile_columns(int D) { return D <= 64 ? 64 : 128; }
 // j <= i + off, off = nk - nq.
 struct Seq {
     int b, q0, nq, k0, nk;
+    int id;                              // its number: of the batch element, or among the packed ones
     __device__ __forceinline__ int off() const { return nk - nq; }
 };
 
@@ -37,6 +38,7 @@ __device__ __forceinline__ void clipped(const int* cu, int s, int n, int& start,
 }
 __device__ __forceinline__ Seq seq_of(const CParams& p, int s) {
     Seq r;
+    r.id = s;
     if (p.cu_q == nullptr) {
         r.b = s;
         r.q0 = r.k0 = 0;

@@ -47,16 +47,88 @@ struct BwdParams {
     int splits;               // shares of a unit's walk
     const float* lse;
     const float* delta;
+    const float* factor;      // fp16: of dS, for every sequence (see ds_factor)
     float* part0;             // splits > 1: [splits][B rows heads][D] partial dQ, or dK
     float* part1;             // dV
     DeviceStatus* status;
     uint64_t wait_limit_ns;
 };
 
-// Delta, eight elements a lane.
+// fp16 keeps all of its bits from 2^-14 to 2^16 only.  Over n keys P is about 1 / n and dS that times the size of dO and V, so as they
+// are both would lose bits or vanish although the gradients do not (dQ off by 3 % at 4096 keys and |dO| = 10^-3, by 29 % at
+// 10^-4).  P therefore goes into dV times 2^15, and dS into dQ and dK without the softmax scale and times a power of two of its
+// sequence, as large as overflow allows; both are undone in fp32 where rows are written.  (bf16 has the exponents of fp32: nothing
+// of this.)  With M the largest |dO_i . V_j| of a sequence, |dS_ij| = P_ij |sum_k P_ik (dP_ij - dP_ik)| <= 2 M P_ij (1 - P_ij) <= M / 2,
+// and M is at most the product of the longest rows of dO and V.  For rows of normal values the factor makes dS about 2^13 P.
+constexpr float kPFactor = 32768.f, kPFactorLog2 = 15.f;
+// from the squares of the two lengths: a power of two f with sqrt(do2 v2) / 2 f in [2^14, 2^15)
+__device__ __forceinline__ float ds_factor(float do2, float v2) {
+    const float x = do2 * v2;                          // (2^-96 to 2^79)
+    if (!(x > 0.f)) return 1.f;
+    const int e = (__float_as_int(x) >> 23) - 127;     // x < 2^(e + 1)
+    return __int_as_float((16 - ((e + 2) >> 1) + 127) << 23);
+}
+
+// Squares of the longest rows of dO and V of every sequence, without elements that are not finite (their rows' gradients are not
+// either) and queries that see nothing: `parts` blocks for a sequence, joined by the Delta kernel.
+template <int HD>
+__global__ void __launch_bounds__(256) causal_norms_kernel(const CParams p, const __nv_bfloat16* __restrict__ v, const __nv_bfloat16* __restrict__ d_o,
+                                                          float2* __restrict__ norms, int parts) {
+    using E = ptx::El<true>;
+    constexpr int kLanes = HD / 8, kRows = 256 / kLanes, kUnroll = 4;
+    __shared__ float tops[2][8];
+    const int lane = threadIdx.x % kLanes, row0 = threadIdx.x / kLanes;
+    const Seq s = seq_of(p, blockIdx.x / parts);
+    const unsigned part = blockIdx.x % parts;
+    auto longest = [&](const __nv_bfloat16* x, const sa_strides& st, int first, int rows, unsigned heads) {
+        const unsigned total = (unsigned)max(rows - first, 0) * heads;         // (rows fit 31 bits)
+        float top = 0.f;
+        x += s.b * st.b + 8 * lane;
+        for (unsigned r0 = part * kRows * kUnroll; r0 < total; r0 += parts * kRows * kUnroll) {
+            uint4 w[kUnroll];
+#pragma unroll
+            for (int y = 0; y < kUnroll; ++y) {
+                const unsigned r = r0 + y * kRows + row0, i = r / heads;
+                w[y] = make_uint4(0, 0, 0, 0);
+                if (r < total && 8 * lane < p.D) w[y] = *reinterpret_cast<const uint4*>(x + (int64_t)(first + (int)i) * st.n + (r - i * heads) * st.h);
+            }
+#pragma unroll
+            for (int y = 0; y < kUnroll; ++y) {
+                const uint32_t word[4] = {w[y].x, w[y].y, w[y].z, w[y].w};
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a = E::lo(word[e]), b = E::hi(word[e]);
+                    if (fabsf(a) < INFINITY) sum = fmaf(a, a, sum);
+                    if (fabsf(b) < INFINITY) sum = fmaf(b, b, sum);
+                }
+#pragma unroll
+                for (int z = kLanes / 2; z > 0; z >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, z);
+                top = fmaxf(top, sum);
+            }
+        }
+#pragma unroll
+        for (int z = 16; z > 0; z >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, z));
+        return top;
+    };
+    const float a = longest(d_o + s.q0 * p.d_o.n, p.d_o, max(-s.off(), 0), s.nq, p.H), b = longest(v + s.k0 * p.v.n, p.v, 0, s.nk, p.Hkv);
+    if ((threadIdx.x & 31) == 0) {
+        tops[0][threadIdx.x >> 5] = a;
+        tops[1][threadIdx.x >> 5] = b;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float2 t = make_float2(0.f, 0.f);
+        for (int y = 0; y < 8; ++y) t = make_float2(fmaxf(t.x, tops[0][y]), fmaxf(t.y, tops[1][y]));
+        norms[blockIdx.x] = t;
+    }
+}
+
+// Delta, eight elements a lane; for fp16 also the sequences' factors of dS.
 template <int HD, bool F16>
 __global__ void __launch_bounds__(256) causal_delta16_kernel(const CParams p, const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o_low,
-                                                            const __nv_bfloat16* __restrict__ d_o, float* __restrict__ delta) {
+                                                            const __nv_bfloat16* __restrict__ d_o, float* __restrict__ delta, const float2* __restrict__ norms,
+                                                            int parts, float* __restrict__ factor) {
     using E = ptx::El<F16>;
     constexpr int kLanes = HD / 8;
     const int lane = threadIdx.x % kLanes;
@@ -85,6 +157,19 @@ __global__ void __launch_bounds__(256) causal_delta16_kernel(const CParams p, co
 #pragma unroll
     for (int s = kLanes / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
     if (in && lane == 0) delta[((int64_t)b * p.H + h) * p.Nq + i] = sum;
+    if constexpr (F16) {
+        if (threadIdx.x < 32)
+            for (int s = blockIdx.x; s < p.S; s += gridDim.x) {
+                float2 t = make_float2(0.f, 0.f);
+                for (int y = threadIdx.x; y < parts; y += 32) {
+                    const float2 z = norms[(int64_t)s * parts + y];
+                    t = make_float2(fmaxf(t.x, z.x), fmaxf(t.y, z.y));
+                }
+#pragma unroll
+                for (int z = 16; z > 0; z >>= 1) t = make_float2(fmaxf(t.x, __shfl_xor_sync(0xffffffffu, t.x, z)), fmaxf(t.y, __shfl_xor_sync(0xffffffffu, t.y, z)));
+                if (threadIdx.x == 0) factor[s] = ds_factor(t.x, t.y);
+            }
+    }
 }
 
 // Units in the order of the work list, a block's rounds in alternating direction.
@@ -326,6 +411,7 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
                 for (int it = 0; it < u.n; ++it, st.next(u)) {
                     const int i0 = st.i0(u), h = u.hk * p.G + st.g;
                     const int64_t at = ((int64_t)u.s.b * p.H + h) * p.Nq + u.s.q0 + i0;
+                    const float f = F16 ? P.factor[u.s.id] / kPFactor : p.scale;
                     float ls[4], dl[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -333,8 +419,8 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
                         ls[e] = INFINITY;              // a row that does not exist, or sees nothing: P = exp2(-inf) = 0
                         dl[e] = 0.f;
                         if (i0 + i < u.s.nq && i0 + i + u.s.off() >= 0) {
-                            ls[e] = P.lse[at + i] * kLog2e;
-                            dl[e] = P.delta[at + i] * p.scale;
+                            ls[e] = P.lse[at + i] * kLog2e - (F16 ? kPFactorLog2 : 0.f);
+                            dl[e] = P.delta[at + i] * f;
                         }
                     }
                     mbar_wait<kFull>(base + 8 * g.s, g.phase, wctx, 9);
@@ -361,12 +447,14 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
         const int grp = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(row & ~31) << 16;
         const uint32_t s_addr = tm_s + lanes + 64 * grp, dp_addr = tm_dp + lanes + 64 * grp;
-        const float2 c2 = make_float2(p.scale * kLog2e, p.scale * kLog2e), sc = make_float2(p.scale, p.scale);
+        const float2 c2 = make_float2(p.scale * kLog2e, p.scale * kLog2e);
         Ring g;
         uint32_t n = 0, nu = 0;
         for (Walk w(P, p.Hkv); w.valid(); w.next()) {
             const ColUnit u = col_unit(P, w);
             ColStep st(u);
+            const float f = F16 ? P.factor[u.s.id] / kPFactor : p.scale;        // of dP; P has 2^15 already (through its LSE)
+            const float2 sc = make_float2(f, f);
 #pragma unroll 1
             for (int it = 0; it < u.n; ++it, ++n, st.next(u)) {
                 const int i0 = st.i0(u);
@@ -457,6 +545,7 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
                 tc_fence_after();
                 ++nu;
             }
+            const float undo = grp ? p.scale / (f * kPFactor) : 1.f / kPFactor;
             __nv_bfloat16* const dst = out + u.s.b * so.b + (int64_t)(u.s.k0 + u.j0 + row) * so.n + u.hk * so.h;
             float* const pdst = part + (((int64_t)u.split * p.B + u.s.b) * p.Hkv + u.hk) * (int64_t)p.Nk * HD + (int64_t)(u.s.k0 + u.j0 + row) * HD;
 #pragma unroll 1
@@ -470,6 +559,10 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
                     for (int e = 0; e < 32; ++e) x[e] = 0u;
                 }
                 if (!mine) continue;
+                if constexpr (F16) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * undo);
+                }
                 if (P.splits > 1) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(pdst + c0 + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
@@ -786,17 +879,19 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
         reg_alloc<kRowRegsCompute>();
         const int grp = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(row & ~31) << 16;
-        const float2 c2 = make_float2(p.scale * kLog2e, p.scale * kLog2e), sc = make_float2(p.scale, p.scale);
+        const float2 c2 = make_float2(p.scale * kLog2e, p.scale * kLog2e);
         uint32_t n = 0, nu = 0, n3 = 0;
         for (Walk w(P, p.H); w.valid(); w.next()) {
             const RowUnit u = row_unit(P, w);
             const int i = u.i0 + row;
             const bool mine = i < u.s.nq;
             const int64_t at = ((int64_t)u.s.b * p.H + u.h) * p.Nq + u.s.q0 + i;
+            const float f = F16 ? P.factor[u.s.id] : p.scale;
+            const float2 sc = make_float2(f, f);
             float ls = -INFINITY, dl = 0.f;              // (negated: P = exp2(S c2 + ls); a row that sees nothing has P = 0)
             if (mine && i + u.s.off() >= 0) {
                 ls = -P.lse[at] * kLog2e;
-                dl = -P.delta[at] * p.scale;
+                dl = -P.delta[at] * f;
             }
             const float2 nls = make_float2(ls, ls), ndl = make_float2(dl, dl);
             const int masked_from = u.first_masked();
@@ -864,6 +959,11 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                     for (int e = 0; e < 16; ++e) x[e] = 0u;
                 }
                 if (!mine) continue;
+                if constexpr (F16) {
+                    const float undo = p.scale / f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * undo);
+                }
                 if (P.splits > 1) {
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(part + c0 + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
@@ -932,9 +1032,10 @@ int launch_add(bool f16, const float* part, void* out, const sa_strides& so, int
 struct BwdPlan {
     int64_t items_q, items_k;         // at most
     int splits_q, splits_k;
-    size_t delta, list_q, list_k, part_q, part_k, part_v, bytes;
+    int parts;                        // fp16: of a sequence, for the norms
+    size_t delta, list_q, list_k, part_q, part_k, part_v, norms, factor, bytes;
 };
-inline BwdPlan plan_bwd(const CParams& c) {
+inline BwdPlan plan_bwd(const CParams& c, bool f16) {
     BwdPlan f{};
     const bool packed = c.cu_q != nullptr;
     f.items_q = packed ? list_capacity(c.Nq, kTile, c.S) : (int64_t)ceil_div(c.Nq, kTile) * c.S;
@@ -955,6 +1056,12 @@ inline BwdPlan plan_bwd(const CParams& c) {
     f.part_q = take(f.splits_q > 1 ? (size_t)f.splits_q * c.B * c.H * c.Nq * tile_columns(c.D) * 4 : 0);
     f.part_k = take(f.splits_k > 1 ? (size_t)f.splits_k * c.B * c.Hkv * c.Nk * tile_columns(c.D) * 4 : 0);
     f.part_v = take(f.splits_k > 1 ? (size_t)f.splits_k * c.B * c.Hkv * c.Nk * tile_columns(c.D) * 4 : 0);
+    // (blocks that fill the multiprocessors, with a few rows a thread)
+    const int64_t blocks = ((int64_t)c.B * c.H * c.Nq + (int64_t)c.B * c.Hkv * c.Nk) / (128LL * c.S) + 1;
+    f.parts = (int)(blocks < 256 ? blocks : 256);
+    if (f.parts > ceil_div(8 * sms, c.S)) f.parts = ceil_div(8 * sms, c.S);
+    f.norms = take(f16 ? (size_t)c.S * f.parts * sizeof(float2) : 0);
+    f.factor = take(f16 ? (size_t)c.S * sizeof(float) : 0);
     f.bytes = at;
     return f;
 }
@@ -962,7 +1069,7 @@ inline BwdPlan plan_bwd(const CParams& c) {
 template <int HD, bool F16>
 int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v, const void* o, const void* o_low, const float* lse, const void* d_o,
                   void* dq, void* dk, void* dv, uint8_t* ws, DeviceStatus* status, cudaStream_t st) {
-    const BwdPlan f = plan_bwd(c);
+    const BwdPlan f = plan_bwd(c, F16);
     if (f.items_q * c.H * f.splits_q > 0x3fffffff || f.items_k * c.Hkv * f.splits_k > 0x3fffffff) return SA_ERR_UNSUPPORTED;
     CUtensorMap mq, mk, mv, mo;
     if (!host::make_map(&mq, q, c.B, c.Nq, c.H, c.D, c.q, kTile, F16) || !host::make_map(&mk, k, c.B, c.Nk, c.Hkv, c.D, c.k, kTile, F16) ||
@@ -974,13 +1081,21 @@ int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v,
     float* delta = reinterpret_cast<float*>(ws + f.delta);
     const int64_t rows = (int64_t)c.B * c.Nq * c.H;
     constexpr int kPerBlock = 256 / (HD / 8);
+    float2* const norms = reinterpret_cast<float2*>(ws + f.norms);
+    float* const factor = reinterpret_cast<float*>(ws + f.factor);
+    if constexpr (F16) {
+        if ((int64_t)c.S * f.parts > 0x7fffffff) return SA_ERR_UNSUPPORTED;
+        causal_norms_kernel<HD><<<(unsigned)(c.S * f.parts), 256, 0, st>>>(c, (const __nv_bfloat16*)v, (const __nv_bfloat16*)d_o, norms, f.parts);
+        host::count_launches(1);
+    }
     causal_delta16_kernel<HD, F16><<<(unsigned)((rows + kPerBlock - 1) / kPerBlock), 256, 0, st>>>(c, (const __nv_bfloat16*)o, (const __nv_bfloat16*)o_low,
-                                                                                                     (const __nv_bfloat16*)d_o, delta);
+                                                                                                     (const __nv_bfloat16*)d_o, delta, norms, f.parts, factor);
     host::count_launches(1);
     BwdParams P{};
     P.c = c;
     P.lse = lse;
     P.delta = delta;
+    P.factor = factor;
     P.status = status;
     P.wait_limit_ns = host::wait_limit_ns();
     P.work.S = c.S;

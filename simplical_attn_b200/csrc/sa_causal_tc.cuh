@@ -39,8 +39,8 @@ __device__ __forceinline__ void make_uniform(int& x) { x = uniform(x); }
 // One entry of a packed batch's list of work: a tile of a sequence.
 struct alignas(32) Item {
     int q0, nq, k0, nk;
-    int tile;
-    int pad[3];
+    int tile, seq;
+    int pad[2];
 };
 struct alignas(32) ListHead {
     int count;
@@ -68,9 +68,10 @@ __device__ __forceinline__ void list_item(const CParams& p, const WorkList& w, i
         s.k0 = min(max(a.z, 0), p.Nk);
         s.nk = min(max(a.w, 0), p.Nk - s.k0);
         tile = min(max(e->tile, 0), 1 << 23);
+        s.id = min(max(e->seq, 0), p.S - 1);
     } else {
         tile = i / w.S;
-        s.b = i - tile * w.S;
+        s.b = s.id = i - tile * w.S;
         s.q0 = s.k0 = 0;
         s.nq = p.Nq;
         s.nk = p.Nk;
@@ -147,6 +148,7 @@ __global__ void __launch_bounds__(1024) causal_plan_kernel(const CParams p, cons
         Item* e = items + at;
         *reinterpret_cast<int4*>(e) = make_int4(q.q0, q.nq, q.k0, q.nk);
         e->tile = tile;
+        e->seq = q.id;
     });
 }
 
