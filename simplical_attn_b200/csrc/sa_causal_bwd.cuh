@@ -11,8 +11,8 @@
 // Both are persistent, with groups of four warps (compute) each at a share of a tile's columns and a row of tensor memory per
 // thread -- two groups (dK, dV) or four (dQ: 700 -> 580 us at D = 64 of the size below; for dK, dV no difference) --, then a warp
 // issuing MMAs, one TMA loads, one guarding: it zeroes the rows behind a sequence's end in tiles that
-// the MMAs sum over (they belong to the next sequence, and a masked zero times its NaN would not be zero), and in the dK / dV
-// kernel loads LSE and Delta of the query tile.  P and dS go from registers to tensor memory and from there into the MMA as
+// the MMAs sum over (they belong to the next sequence, and a masked zero times its NaN would not be zero) and the queries that see
+// no key, and in the dK / dV kernel loads LSE and Delta of the query tile.  P and dS go from registers to tensor memory and from there into the MMA as
 // the A operand; a group's packed values lie in the columns of its scores.
 //
 // The streams of tiles run on over units: while the rows of a finished unit are written out, the next one's scores are
@@ -193,11 +193,11 @@ struct Walk {
         if (lane == 0) mbar_arrive<(OFF)>(BASE);   \
     } while (0)
 
-// Zeroes rows [from, 128) of a [128 x HD] tile (a warp).
+// Zeroes the rows of a [128 x HD] tile that are not in [first, from) (a warp).
 template <int HD>
-__device__ __forceinline__ void zero_tile_rows(uint32_t tile, int from, int lane) {
+__device__ __forceinline__ void zero_tile_rows(uint32_t tile, int first, int from, int lane) {
     for (int c = lane; c < kTile * HD / 8; c += 32)
-        if (c / 8 % kTile >= from) ptx::sts128(tile + c * 16, make_uint4(0, 0, 0, 0));
+        if (c / 8 % kTile < first || c / 8 % kTile >= from) ptx::sts128(tile + c * 16, make_uint4(0, 0, 0, 0));
 }
 
 // ---------------------------------------------------------------------------------------------- dK, dV
@@ -430,10 +430,11 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
                         sts_f32(stats + (32 * e + lane) * 4, ls[e]);
                         sts_f32(stats + (kTile + 32 * e + lane) * 4, dl[e]);
                     }
-                    if (i0 + kTile > u.s.nq) {
+                    const int blind = -(i0 + u.s.off());        // rows before it see no key (there are some if queries outnumber keys)
+                    if (i0 + kTile > u.s.nq || blind > 0) {
                         const uint32_t tile = base + L::kRing + g.s * 2 * L::kTileBytes;
-                        zero_tile_rows<HD>(tile, u.s.nq - i0, lane);
-                        zero_tile_rows<HD>(tile + L::kTileBytes, u.s.nq - i0, lane);
+                        zero_tile_rows<HD>(tile, blind, u.s.nq - i0, lane);
+                        zero_tile_rows<HD>(tile + L::kTileBytes, blind, u.s.nq - i0, lane);
                         fence_proxy_async_smem();
                     }
                     SA_ARRIVE(kPassed, base + 8 * g.s);
@@ -866,7 +867,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 mbar_wait<kKFull>(base + 8 * g.s, g.phase, wctx, 13);
                 const int rows = x.u.s.nk - (x.u.t0 + x.t) * kTile;
                 if (rows < kTile) {
-                    zero_tile_rows<HD>(base + L::kKRing + g.s * L::kTileBytes, rows, lane);
+                    zero_tile_rows<HD>(base + L::kKRing + g.s * L::kTileBytes, 0, rows, lane);
                     fence_proxy_async_smem();
                 }
                 SA_ARRIVE(kPassed, base + 8 * g.s);
@@ -884,12 +885,12 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
         for (Walk w(P, p.H); w.valid(); w.next()) {
             const RowUnit u = row_unit(P, w);
             const int i = u.i0 + row;
-            const bool mine = i < u.s.nq;
+            const bool mine = i < u.s.nq, sees = i + u.s.off() >= 0;
             const int64_t at = ((int64_t)u.s.b * p.H + u.h) * p.Nq + u.s.q0 + i;
             const float f = F16 ? P.factor[u.s.id] : p.scale;
             const float2 sc = make_float2(f, f);
             float ls = -INFINITY, dl = 0.f;              // (negated: P = exp2(S c2 + ls); a row that sees nothing has P = 0)
-            if (mine && i + u.s.off() >= 0) {
+            if (mine && sees) {
                 ls = -P.lse[at] * kLog2e;
                 dl = -P.delta[at] * f;
             }
@@ -954,7 +955,8 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 if (u.n > 0) {
                     tmem_ld16(tm_dq + lanes + col + c0, x);
                     tmem_wait_ld();
-                } else {
+                }
+                if (u.n == 0 || !sees) {           // (zero, whatever the row's masked zeros met in K)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[e] = 0u;
                 }
