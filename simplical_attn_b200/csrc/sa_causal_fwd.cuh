@@ -538,7 +538,9 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         const bool up = bad[c0 + e] <= limit, down = bad[HD + c0 + e] <= limit, nan = bad[2 * HD + c0 + e] <= limit;
-                        if (up || down || nan) x[e] = nan || (up && down) ? 0x7fc00000u : up ? 0x7f800000u : 0xff800000u;
+                        // (added: a row that is NaN or the other infinity already, through earlier keys or Q, becomes or stays NaN)
+                        if (up || down || nan)
+                            x[e] = __float_as_uint(__uint_as_float(x[e]) + __uint_as_float(nan || (up && down) ? 0x7fc00000u : up ? 0x7f800000u : 0xff800000u));
                     }
                 }
                 if (mine) {

@@ -1,0 +1,43 @@
+"""Causal attention where a column of V holds several kinds of values that are not finite."""
+import math
+
+import pytest
+import torch
+
+import simplical_attn_b200 as sab
+from tests.test_causal import algo, make  # noqa: F401 (algo: fixture)
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("D,dtype", [(64, "bf16"), (128, "fp16"), (48, "fp32")])
+@pytest.mark.parametrize("B,H,N", [(1, 2, 300), (5, 32, 300)])
+def test_several_kinds_in_a_column(D, dtype, B, H, N, algo):  # noqa: F811
+    """An infinity does not hide the NaN or the opposite infinity of an earlier key: their sum is NaN, as in the definition."""
+    (q, k, v, _), _, _ = make([(N, N)] * B, H, H, D, dtype, seed=52)
+    q, k, v = (t.view(B, N, H, D) for t in (q, k, v))
+    clean = sab.causal_attention(q, k, v)
+    for first, value in ((3, math.nan), (7, -math.inf)):
+        for d in (first, first + 20):
+            v[:, 10, :, d] = value
+            v[:, 270 if d == first else 100, :, d] = math.inf
+    got = sab.causal_attention(q, k, v)
+    for d, early, late in ((3, math.nan, 270), (23, math.nan, 100), (7, -math.inf, 270), (27, -math.inf, 100)):
+        assert torch.equal(got[:, :10, :, d], clean[:, :10, :, d])
+        x = got[:, 10:late, :, d]
+        assert torch.isnan(x).all() if math.isnan(early) else (x == early).all(), d
+        assert torch.isnan(got[:, late:, :, d]).all(), d
+    keep = [d for d in range(D) if d not in (3, 23, 7, 27)]
+    assert torch.equal(got[..., keep], clean[..., keep])
+
+
+@gpu
+@pytest.mark.parametrize("D,dtype", [(64, "bf16"), (128, "fp16")])
+def test_a_row_that_is_not_finite_stays_so(D, dtype, algo):  # noqa: F811
+    """A NaN in Q makes the whole row NaN, an infinity in a column of V notwithstanding."""
+    (q, k, v, _), (cu_q, cu_k), _ = make([(300, 300)], 2, 1, D, dtype, seed=53)
+    q[290, :, 0] = math.nan
+    v[280, :, 5] = math.inf
+    got = sab.causal_attention(q, k, v, cu_q=cu_q, cu_k=cu_k)
+    assert torch.isnan(got[290]).all() and (got[280:290, :, 5] == math.inf).all() and (got[291:, :, 5] == math.inf).all()
