@@ -47,7 +47,8 @@ struct BwdParams {
     int splits;               // shares of a unit's walk
     const float* lse;
     const float* delta;
-    const float* factor;      // fp16: of dS, for every sequence (see ds_factor)
+    const float2* norms;      // fp16: [sequence][parts] (see ds_factor)
+    int parts;
     float* part0;             // splits > 1: [splits][B rows heads][D] partial dQ, or dK
     float* part1;             // dV
     DeviceStatus* status;
@@ -61,8 +62,17 @@ struct BwdParams {
 // of this.)  With M the largest |dO_i . V_j| of a sequence, |dS_ij| = P_ij |sum_k P_ik (dP_ij - dP_ik)| <= 2 M P_ij (1 - P_ij) <= M / 2,
 // and M is at most the product of the longest rows of dO and V.  For rows of normal values the factor makes dS about 2^13 P.
 constexpr float kPFactor = 32768.f, kPFactorLog2 = 15.f;
-// from the squares of the two lengths: a power of two f with sqrt(do2 v2) / 2 f in [2^14, 2^15)
-__device__ __forceinline__ float ds_factor(float do2, float v2) {
+// The factor of a sequence (a whole warp): from the squares of the two lengths a power of two f with sqrt(do2 v2) / 2 f in [2^14, 2^15).
+__device__ __forceinline__ float ds_factor(const BwdParams& P, int sequence) {
+    float do2 = 0.f, v2 = 0.f;
+    for (int y = threadIdx.x & 31; y < P.parts; y += 32) {
+        const float2 t = P.norms[(int64_t)sequence * P.parts + y];
+        do2 = fmaxf(do2, t.x);
+        v2 = fmaxf(v2, t.y);
+    }
+    // (not negative: ordered as their bits are)
+    do2 = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(do2)));
+    v2 = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v2)));
     const float x = do2 * v2;                          // (2^-96 to 2^79)
     if (!(x > 0.f)) return 1.f;
     const int e = (__float_as_int(x) >> 23) - 127;     // x < 2^(e + 1)
@@ -70,10 +80,10 @@ __device__ __forceinline__ float ds_factor(float do2, float v2) {
 }
 
 // Squares of the longest rows of dO and V of every sequence, without elements that are not finite (their rows' gradients are not
-// either) and queries that see nothing: `parts` blocks for a sequence, joined by the Delta kernel.
+// either) and queries that see nothing: `parts` blocks for a sequence.
 template <int HD>
-__global__ void __launch_bounds__(256) causal_norms_kernel(const CParams p, const __nv_bfloat16* __restrict__ v, const __nv_bfloat16* __restrict__ d_o,
-                                                          float2* __restrict__ norms, int parts) {
+__device__ __forceinline__ void longest_rows(const CParams& p, const __nv_bfloat16* __restrict__ v, const __nv_bfloat16* __restrict__ d_o,
+                                             float2* __restrict__ norms, int parts) {
     using E = ptx::El<true>;
     constexpr int kLanes = HD / 8, kRows = 256 / kLanes, kUnroll = 4;
     __shared__ float tops[2][8];
@@ -124,16 +134,25 @@ __global__ void __launch_bounds__(256) causal_norms_kernel(const CParams p, cons
     }
 }
 
-// Delta, eight elements a lane; for fp16 also the sequences' factors of dS.
+// Delta, eight elements a lane; for fp16 the first blocks find the sequences' longest rows.
 template <int HD, bool F16>
 __global__ void __launch_bounds__(256) causal_delta16_kernel(const CParams p, const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o_low,
-                                                            const __nv_bfloat16* __restrict__ d_o, float* __restrict__ delta, const float2* __restrict__ norms,
-                                                            int parts, float* __restrict__ factor) {
+                                                            const __nv_bfloat16* __restrict__ v, const __nv_bfloat16* __restrict__ d_o, float* __restrict__ delta,
+                                                            float2* __restrict__ norms, int parts) {
     using E = ptx::El<F16>;
     constexpr int kLanes = HD / 8;
     const int lane = threadIdx.x % kLanes;
     // (rows fit 31 bits; 64-bit divisions took most of this kernel's time)
-    const unsigned w = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+    unsigned block = blockIdx.x;
+    if constexpr (F16) {
+        const unsigned first = (unsigned)p.S * (unsigned)parts;
+        if (block < first) {
+            longest_rows<HD>(p, v, d_o, norms, parts);
+            return;
+        }
+        block -= first;
+    }
+    const unsigned w = block * (256 / kLanes) + threadIdx.x / kLanes;
     float sum = 0.f;
     int h = 0, i = 0, b = 0;
     const bool in = w < (unsigned)(p.B * p.Nq * p.H);
@@ -157,19 +176,6 @@ __global__ void __launch_bounds__(256) causal_delta16_kernel(const CParams p, co
 #pragma unroll
     for (int s = kLanes / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
     if (in && lane == 0) delta[((int64_t)b * p.H + h) * p.Nq + i] = sum;
-    if constexpr (F16) {
-        if (threadIdx.x < 32)
-            for (int s = blockIdx.x; s < p.S; s += gridDim.x) {
-                float2 t = make_float2(0.f, 0.f);
-                for (int y = threadIdx.x; y < parts; y += 32) {
-                    const float2 z = norms[(int64_t)s * parts + y];
-                    t = make_float2(fmaxf(t.x, z.x), fmaxf(t.y, z.y));
-                }
-#pragma unroll
-                for (int z = 16; z > 0; z >>= 1) t = make_float2(fmaxf(t.x, __shfl_xor_sync(0xffffffffu, t.x, z)), fmaxf(t.y, __shfl_xor_sync(0xffffffffu, t.y, z)));
-                if (threadIdx.x == 0) factor[s] = ds_factor(t.x, t.y);
-            }
-    }
 }
 
 // Units in the order of the work list, a block's rounds in alternating direction.
@@ -408,10 +414,10 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
             for (Walk w(P, p.Hkv); w.valid(); w.next()) {
                 const ColUnit u = col_unit(P, w);
                 ColStep st(u);
+                const float f = F16 ? ds_factor(P, u.s.id) / kPFactor : p.scale;
                 for (int it = 0; it < u.n; ++it, st.next(u)) {
                     const int i0 = st.i0(u), h = u.hk * p.G + st.g;
                     const int64_t at = ((int64_t)u.s.b * p.H + h) * p.Nq + u.s.q0 + i0;
-                    const float f = F16 ? P.factor[u.s.id] / kPFactor : p.scale;
                     float ls[4], dl[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -454,7 +460,7 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
         for (Walk w(P, p.Hkv); w.valid(); w.next()) {
             const ColUnit u = col_unit(P, w);
             ColStep st(u);
-            const float f = F16 ? P.factor[u.s.id] / kPFactor : p.scale;        // of dP; P has 2^15 already (through its LSE)
+            const float f = F16 ? ds_factor(P, u.s.id) / kPFactor : p.scale;        // of dP; P has 2^15 already (through its LSE)
             const float2 sc = make_float2(f, f);
 #pragma unroll 1
             for (int it = 0; it < u.n; ++it, ++n, st.next(u)) {
@@ -887,7 +893,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
             const int i = u.i0 + row;
             const bool mine = i < u.s.nq, sees = i + u.s.off() >= 0;
             const int64_t at = ((int64_t)u.s.b * p.H + u.h) * p.Nq + u.s.q0 + i;
-            const float f = F16 ? P.factor[u.s.id] : p.scale;
+            const float f = F16 ? ds_factor(P, u.s.id) : p.scale;
             const float2 sc = make_float2(f, f);
             float ls = -INFINITY, dl = 0.f;              // (negated: P = exp2(S c2 + ls); a row that sees nothing has P = 0)
             if (mine && sees) {
@@ -1035,7 +1041,7 @@ struct BwdPlan {
     int64_t items_q, items_k;         // at most
     int splits_q, splits_k;
     int parts;                        // fp16: of a sequence, for the norms
-    size_t delta, list_q, list_k, part_q, part_k, part_v, norms, factor, bytes;
+    size_t delta, list_q, list_k, part_q, part_k, part_v, norms, bytes;
 };
 inline BwdPlan plan_bwd(const CParams& c, bool f16) {
     BwdPlan f{};
@@ -1063,7 +1069,6 @@ inline BwdPlan plan_bwd(const CParams& c, bool f16) {
     f.parts = (int)(blocks < 256 ? blocks : 256);
     if (f.parts > ceil_div(8 * sms, c.S)) f.parts = ceil_div(8 * sms, c.S);
     f.norms = take(f16 ? (size_t)c.S * f.parts * sizeof(float2) : 0);
-    f.factor = take(f16 ? (size_t)c.S * sizeof(float) : 0);
     f.bytes = at;
     return f;
 }
@@ -1084,20 +1089,17 @@ int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v,
     const int64_t rows = (int64_t)c.B * c.Nq * c.H;
     constexpr int kPerBlock = 256 / (HD / 8);
     float2* const norms = reinterpret_cast<float2*>(ws + f.norms);
-    float* const factor = reinterpret_cast<float*>(ws + f.factor);
-    if constexpr (F16) {
-        if ((int64_t)c.S * f.parts > 0x7fffffff) return SA_ERR_UNSUPPORTED;
-        causal_norms_kernel<HD><<<(unsigned)(c.S * f.parts), 256, 0, st>>>(c, (const __nv_bfloat16*)v, (const __nv_bfloat16*)d_o, norms, f.parts);
-        host::count_launches(1);
-    }
-    causal_delta16_kernel<HD, F16><<<(unsigned)((rows + kPerBlock - 1) / kPerBlock), 256, 0, st>>>(c, (const __nv_bfloat16*)o, (const __nv_bfloat16*)o_low,
-                                                                                                     (const __nv_bfloat16*)d_o, delta, norms, f.parts, factor);
+    const int64_t delta_blocks = (rows + kPerBlock - 1) / kPerBlock + (F16 ? (int64_t)c.S * f.parts : 0);
+    if (delta_blocks > 0x7fffffff) return SA_ERR_UNSUPPORTED;
+    causal_delta16_kernel<HD, F16><<<(unsigned)delta_blocks, 256, 0, st>>>(c, (const __nv_bfloat16*)o, (const __nv_bfloat16*)o_low, (const __nv_bfloat16*)v,
+                                                                           (const __nv_bfloat16*)d_o, delta, norms, f.parts);
     host::count_launches(1);
     BwdParams P{};
     P.c = c;
     P.lse = lse;
     P.delta = delta;
-    P.factor = factor;
+    P.norms = norms;
+    P.parts = f.parts;
     P.status = status;
     P.wait_limit_ns = host::wait_limit_ns();
     P.work.S = c.S;
