@@ -342,10 +342,8 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
                 constexpr uint32_t kExp = F16 ? 0x7c00u : 0x7f80u;
                 if (*bad_unit != (int)units + 1) {
                     // what is noted now may still be wanted by rows of earlier units: they are written out first
-                    const uint64_t began = globaltimer_ns();
-                    while ((done[0] < (int)units || done[1] < (int)units) && !lds_volatile(wctx.abort_flag) && globaltimer_ns() - began < wctx.limit_ns) {
-                    }
-                    __syncwarp();
+                    auto written = [&] { return done[0] >= (int)units && done[1] >= (int)units; };
+                    if (!__all_sync(0xffffffffu, mbar_wait_on(written, written, wctx, 18))) return;
                     for (int d = lane; d < 3 * HD; d += 32) bad[d] = 0x7fffffff;
                     __threadfence_block();
                     __syncwarp();
