@@ -1103,6 +1103,7 @@ int launch_bwd_tc(const CParams& c, const void* q, const void* k, const void* v,
     P.status = status;
     P.wait_limit_ns = host::wait_limit_ns();
     P.work.S = c.S;
+    P.work.last = last_tile(kTile);
     PlanParams plan{};
     if (c.cu_q != nullptr) {
         plan.list[0] = reinterpret_cast<ListHead*>(ws + f.list_q);

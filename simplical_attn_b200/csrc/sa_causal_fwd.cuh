@@ -731,6 +731,7 @@ int launch_fwd_tc(const CParams& c, const void* q, const void* k, const void* v,
     P.part_lse = reinterpret_cast<float*>(ws + f.part_lse);
     P.status = status;
     P.wait_limit_ns = host::wait_limit_ns();
+    P.work.last = last_tile(kTile * f.row_tiles);
     P.work.tiles = ceil_div(c.Nq, kTile * f.row_tiles);
     P.work.S = c.S;
     P.work.descending = 1;

@@ -51,9 +51,14 @@ struct alignas(32) ListHead {
 // ones.  Without a list (batched tensors) tile and sequence follow from the index.
 struct WorkList {
     const ListHead* head;             // NULL: no list; items follow the head
+    int last;                         // with a list: last_tile of its tiles
     int tiles, S;                     // without a list: tiles per sequence, sequences
     int descending;                   // without a list: whether later tiles are the more expensive ones
 };
+
+// The last tile of so many rows that a tensor of the most rows that a call may have (2^30) can hold: its first row fits an int.
+constexpr int last_tile(int rows) { return ((1 << 30) - 1) / rows; }
+static_assert((int64_t)(last_tile(kTile) + 1) * kTile <= 1 << 30 && (int64_t)(last_tile(2 * kTile) + 1) * 2 * kTile <= 1 << 30, "rows of listed tiles");
 
 __device__ __forceinline__ int list_count(const WorkList& w) { return w.head ? w.head->count : w.tiles * w.S; }
 
@@ -61,13 +66,13 @@ __device__ __forceinline__ void list_item(const CParams& p, const WorkList& w, i
     if (w.head) {
         const Item* e = reinterpret_cast<const Item*>(w.head + 1) + i;
         const int4 a = *reinterpret_cast<const int4*>(e);
-        // (clipped again: starts that decrease may leave entries of the list unwritten)
+        // (clipped again: starts that are written to while the list is made may leave entries of it as they were)
         s.b = 0;
         s.q0 = min(max(a.x, 0), p.Nq);
         s.nq = min(max(a.y, 0), p.Nq - s.q0);
         s.k0 = min(max(a.z, 0), p.Nk);
         s.nk = min(max(a.w, 0), p.Nk - s.k0);
-        tile = min(max(e->tile, 0), 1 << 23);
+        tile = min(max(e->tile, 0), w.last);
         s.id = min(max(e->seq, 0), p.S - 1);
     } else {
         tile = i / w.S;
