@@ -23,6 +23,11 @@ from .rotary import RotaryPositions
 from .simplicial_attn import two_simplicial_attention
 
 
+def _check_positions(module, positions):
+    if positions is not None and module.rotary is None:
+        raise ValueError("positions are for the rotation of queries and keys: the module was made without rotary")
+
+
 class TwoSimplicialSelfAttention(torch.nn.Module):
     """`y = W_o . attention(W_q x, W_k1 x, W_k2 x, W_v1 x, W_v2 x)` over `[B, N, hidden]` inputs."""
 
@@ -44,6 +49,7 @@ class TwoSimplicialSelfAttention(torch.nn.Module):
         self.out_proj = torch.nn.Linear(num_heads * head_dim, hidden, bias=bias, dtype=dtype, device=device)
 
     def forward(self, x: torch.Tensor, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        _check_positions(self, positions)
         B, N, _ = x.shape
         fused = self.in_proj(x)                                   # one GEMM: [B, N, (H + 4 Hkv) * D]
         parts = torch.split(fused, self.widths, dim=-1)
@@ -77,6 +83,7 @@ class CausalSelfAttention(torch.nn.Module):
 
     def forward(self, x: torch.Tensor, positions: Optional[torch.Tensor] = None, cu: Optional[torch.Tensor] = None,
                 max_len: Optional[int] = None) -> torch.Tensor:
+        _check_positions(self, positions)
         q, k, v = (t.unflatten(-1, (-1, self.head_dim)) for t in torch.split(self.in_proj(x), self.widths, dim=-1))
         if self.rotary is not None:
             q, k = self.rotary(q, k, positions=positions)
