@@ -187,15 +187,16 @@ class RotaryPositions(torch.nn.Module):
         self.rotary_dim = rotary_dim
         self.interleaved = interleaved
         self.magnitude = magnitude
-        self.register_buffer("frequencies", rotary_frequencies(rotary_dim, base, scaling, factor, original_length, low_turns,
-                                                               high_turns, device), persistent=False)
+        self._arguments = (rotary_dim, base, scaling, factor, original_length, low_turns, high_turns)
+        self.register_buffer("frequencies", rotary_frequencies(*self._arguments, device), persistent=False)
 
     def _apply(self, fn, recurse=True):
-        # a cast of the module's parameters (`.to(dtype)`, `.half()`) leaves the frequencies in 64 bits
+        # The values are kept whatever becomes of the parameters: in 64 bits under a cast (`.to(dtype)`, `.half()`), as they are under
+        # `.to_empty()`, which leaves memory unwritten, and from the arguments where they were on the meta device.
         kept = self.frequencies
         super()._apply(fn, recurse)
-        if self.frequencies.dtype != kept.dtype:
-            self.frequencies = kept.to(self.frequencies.device)
+        device = self.frequencies.device
+        self.frequencies = kept.to(device) if device.type == "meta" or not kept.is_meta else rotary_frequencies(*self._arguments, device)
         return self
 
     def forward(self, *tensors, positions: Optional[torch.Tensor] = None, offset: int = 0):
