@@ -231,7 +231,6 @@ void check_causal(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
         TORCH_CHECK_VALUE(cu[i]->dim() == 1 && cu[i]->size(0) >= 2 && cu[i]->size(0) == cu_q.size(0) && cu[i]->is_contiguous(), cu_names[i],
                           " must be contiguous [sequences + 1] with at least one sequence, as many as cu_q has, got ", cu[i]->sizes());
     }
-    TORCH_CHECK_VALUE(!cu_k.is_same(cu_q) || k.size(0) == q.size(0), "without cu_k, k and v must have q's rows");
 }
 
 sa_causal_params causal_params(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& cu_q, const CausalConfig& c) {

@@ -47,8 +47,15 @@ def _check(q, k, v, cu_q, cu_k):
             raise TypeError(f"{name} must be int32 on q's device")
         if cu.dim() != 1 or cu.shape[0] < 2 or cu.shape != cu_q.shape or not cu.is_contiguous():
             raise ValueError(f"{name} must be contiguous [sequences + 1] with at least one sequence, as many as cu_q has")
-    if cu_k is cu_q and k.shape[0] != q.shape[0]:
+
+
+def _starts_of_keys(q, k, cu_q, cu_k):
+    """`cu_k`, which defaults to `cu_q` where the tensors have the same rows."""
+    if cu_k is not None or cu_q is None:
+        return cu_k
+    if k.shape[:1] != q.shape[:1]:
         raise ValueError("without cu_k, k and v must have q's rows")
+    return cu_q
 
 
 def _params(q, k, v, o, cu_q, scale, max_q, max_k, algo):
@@ -72,7 +79,7 @@ def causal_attention_fwd(q, k, v, scale, cu_q=None, cu_k=None, max_q=0, max_k=0,
     """Forward launch: (O, LSE), LSE fp32 [B, H, N] (packed: [H, rows]).  With `low` also what rounding took from a 16-bit O
     (None for fp32), which the backward forms sum dO O with: without it dQ and dK are about 5 % less exact."""
     algo = algo or _host.default_algo
-    cu_k = cu_q if cu_k is None else cu_k
+    cu_k = _starts_of_keys(q, k, cu_q, cu_k)
     if _host._status_watch.active:
         _host._status_watch.poll(q.device)
     native = _native()
@@ -104,7 +111,7 @@ def causal_attention_fwd(q, k, v, scale, cu_q=None, cu_k=None, max_q=0, max_k=0,
 def causal_attention_bwd(q, k, v, o, lse, d_o, scale, cu_q=None, cu_k=None, max_q=0, max_k=0, need=(True, True, True), algo=None, o_low=None):
     """Backward launches: (dq, dk, dv), `None` where `need[i]` is false."""
     algo = algo or _host.default_algo
-    cu_k = cu_q if cu_k is None else cu_k
+    cu_k = _starts_of_keys(q, k, cu_q, cu_k)
     if _host._status_watch.active:
         _host._status_watch.poll(q.device)
     native = _native()
@@ -190,8 +197,7 @@ def causal_attention(q, k, v, scale: Optional[float] = None, *, cu_q: Optional[t
     max_q, max_k = max_q or 0, max_k or 0
     if max_q < 0 or max_k < 0:
         raise ValueError("max_q and max_k must not be negative")
-    if cu_k is None:
-        cu_k = cu_q
+    cu_k = _starts_of_keys(q, k, cu_q, cu_k)
     native = None if _host.debug_device_status else _native()
     if native is not None:
         if _host._status_watch.active:
