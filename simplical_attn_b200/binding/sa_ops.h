@@ -19,7 +19,6 @@ void check_type_of(const Tensor& t) {
 
 // A second backward pass through `grads` raises: the kernels have no derivative of the gradient.
 torch::autograd::variable_list no_second_derivative(torch::autograd::variable_list grads, const char* name) {
-    std::vector<c10::optional<Tensor>> of;
     for (Tensor& g : grads)
         if (g.defined()) g.requires_grad_(true);
     auto error = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " has no second derivative", (int64_t)grads.size());
