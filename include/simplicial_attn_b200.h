@@ -202,8 +202,8 @@ int sa_rotary(const sa_rotary_params* p, const void* const* in, void* const* out
 /* Causal attention over whole prompts, packed sequences, chunks of a prompt or single tokens:
  *     logits_ij = scale * sum_d Q_id * K_jd     over keys j <= i + (keys - queries) of i's sequence
  *     O_i = sum_j softmax_j(logits_i) V_j;      LSE_i = log sum_j exp(logits_ij)
- * so the last query of a sequence sees all its keys.  A query that sees none has O = 0 and LSE = -inf and takes part in no
- * gradient.  Q, O are [B, Nq, H, D], K, V are [B, Nk, Hkv, D], LSE is [B, H, Nq] fp32 contiguous; head h reads KV head
+ * so the last query of a sequence sees all its keys.  A query that sees none, or whose scores are all -inf, has O = 0 and
+ * LSE = -inf and takes part in no gradient.  Q, O are [B, Nq, H, D], K, V are [B, Nk, Hkv, D], LSE is [B, H, Nq] fp32 contiguous; head h reads KV head
  * h / (H / Hkv).
  * sequences == 0: every batch element is a sequence.  Otherwise B == 1 and sequence s is rows [cu_q[s], cu_q[s + 1]) of Q
  * and [cu_k[s], cu_k[s + 1]) of K and V (device memory, `sequences` + 1 ints each, not decreasing; values are clipped to the

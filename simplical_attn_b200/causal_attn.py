@@ -4,7 +4,8 @@
     O_i = sum_j softmax_j(logits_i) V_j
 
 One call serves whole prompts, a chunk of a prompt over the keys before it, single tokens (the last query of a sequence sees
-all its keys) and packed sequences of different lengths, with grouped heads.  A query that sees no key has O = 0.
+all its keys) and packed sequences of different lengths, with grouped heads.  A query that sees no key, or whose scores are
+all -inf, has O = 0.
 The layout is the 2-simplicial operator's: [batch, seq_len, heads, head_dim], or packed [rows, heads, head_dim].
 """
 from __future__ import annotations

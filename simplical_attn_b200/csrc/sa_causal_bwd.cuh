@@ -62,13 +62,20 @@ struct BwdParams {
 // of this.)  With M the largest |dO_i . V_j| of a sequence, |dS_ij| = P_ij |sum_k P_ik (dP_ij - dP_ik)| <= 2 M P_ij (1 - P_ij) <= M / 2,
 // and M is at most the product of the longest rows of dO and V.  For rows of normal values the factor makes dS about 2^13 P.
 constexpr float kPFactor = 32768.f, kPFactorLog2 = 15.f;
+constexpr int kMostParts = 256;
 // The factor of a sequence (a whole warp): from the squares of the two lengths a power of two f with sqrt(do2 v2) / 2 f in [2^14, 2^15).
 __device__ __forceinline__ float ds_factor(const BwdParams& P, int sequence) {
     float do2 = 0.f, v2 = 0.f;
-    for (int y = threadIdx.x & 31; y < P.parts; y += 32) {
-        const float2 t = P.norms[(int64_t)sequence * P.parts + y];
-        do2 = fmaxf(do2, t.x);
-        v2 = fmaxf(v2, t.y);
+    float2 t[kMostParts / 32];
+#pragma unroll
+    for (int x = 0; x < kMostParts / 32; ++x) {        // (all loads under way together: this stands at the start of a unit)
+        const int y = 32 * x + (threadIdx.x & 31);
+        t[x] = y < P.parts ? P.norms[(int64_t)sequence * P.parts + y] : make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int x = 0; x < kMostParts / 32; ++x) {
+        do2 = fmaxf(do2, t[x].x);
+        v2 = fmaxf(v2, t[x].y);
     }
     // (not negative: ordered as their bits are)
     do2 = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(do2)));
@@ -78,6 +85,8 @@ __device__ __forceinline__ float ds_factor(const BwdParams& P, int sequence) {
     const int e = (__float_as_int(x) >> 23) - 127;     // x < 2^(e + 1)
     return __int_as_float((16 - ((e + 2) >> 1) + 127) << 23);
 }
+
+__device__ __forceinline__ float one_over(float power_of_two) { return __int_as_float((254 << 23) - __float_as_int(power_of_two)); }
 
 // Squares of the longest rows of dO and V of every sequence, without elements that are not finite (their rows' gradients are not
 // either) and queries that see nothing: `parts` blocks for a sequence.
@@ -422,14 +431,17 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int i = 32 * e + lane;
-                        ls[e] = INFINITY;              // a row that does not exist, or sees nothing: P = exp2(-inf) = 0
-                        dl[e] = 0.f;
-                        if (i0 + i < u.s.nq && i0 + i + u.s.off() >= 0) {
-                            ls[e] = P.lse[at + i] * kLog2e - (F16 ? kPFactorLog2 : 0.f);
-                            dl[e] = P.delta[at + i] * f;
-                        }
+                        const bool in = i0 + i < u.s.nq && i0 + i + u.s.off() >= 0;
+                        ls[e] = in ? P.lse[at + i] : -INFINITY;
+                        dl[e] = in ? P.delta[at + i] : 0.f;
                     }
                     mbar_wait<kFull>(base + 8 * g.s, g.phase, wctx, 9);
+                    // (a row that does not exist, sees nothing or has scores of -inf only has P = exp2(-inf) = 0)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        dl[e] = ls[e] == -INFINITY ? 0.f : dl[e] * f;
+                        ls[e] = ls[e] == -INFINITY ? INFINITY : ls[e] * kLog2e - (F16 ? kPFactorLog2 : 0.f);
+                    }
                     const uint32_t stats = base + L::kStats + g.s * 2 * kTile * 4;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -552,7 +564,7 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
                 tc_fence_after();
                 ++nu;
             }
-            const float undo = grp ? p.scale / (f * kPFactor) : 1.f / kPFactor;
+            const float undo = grp ? p.scale * one_over(f * kPFactor) : 1.f / kPFactor;
             __nv_bfloat16* const dst = out + u.s.b * so.b + (int64_t)(u.s.k0 + u.j0 + row) * so.n + u.hk * so.h;
             float* const pdst = part + (((int64_t)u.split * p.B + u.s.b) * p.Hkv + u.hk) * (int64_t)p.Nk * HD + (int64_t)(u.s.k0 + u.j0 + row) * HD;
 #pragma unroll 1
@@ -891,15 +903,19 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
         for (Walk w(P, p.H); w.valid(); w.next()) {
             const RowUnit u = row_unit(P, w);
             const int i = u.i0 + row;
-            const bool mine = i < u.s.nq, sees = i + u.s.off() >= 0;
+            const bool mine = i < u.s.nq;
+            const int sees = uniform(u.i0 + u.s.off());      // last key that row 0 sees (below 0: none)
             const int64_t at = ((int64_t)u.s.b * p.H + u.h) * p.Nq + u.s.q0 + i;
+            // (negated: P = exp2(S c2 + ls); a row that sees nothing, or has scores of -inf only, has P = 0.  All loads before what uses them.)
+            float ls = INFINITY, dl = 0.f;
+            if (mine && sees + row >= 0) {
+                ls = -P.lse[at];
+                dl = -P.delta[at];
+            }
             const float f = F16 ? ds_factor(P, u.s.id) : p.scale;
             const float2 sc = make_float2(f, f);
-            float ls = -INFINITY, dl = 0.f;              // (negated: P = exp2(S c2 + ls); a row that sees nothing has P = 0)
-            if (mine && sees) {
-                ls = -P.lse[at] * kLog2e;
-                dl = -P.delta[at] * f;
-            }
+            dl = ls == INFINITY ? 0.f : dl * f;
+            ls = ls == INFINITY ? -INFINITY : ls * kLog2e;
             const float2 nls = make_float2(ls, ls), ndl = make_float2(dl, dl);
             const int masked_from = u.first_masked();
 #pragma unroll 1
@@ -916,7 +932,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 const bool masked = t >= masked_from;
                 uint32_t seen = ~0u;
                 if (masked) {
-                    const int hi = i + u.s.off() - (u.t0 + t) * kTile - kRowCols * grp;        // columns up to this one
+                    const int hi = sees + row - (u.t0 + t) * kTile - kRowCols * grp;        // columns up to this one
                     seen = hi >= 31 ? ~0u : hi < 0 ? 0u : ~0u >> (31 - hi);
                 }
 #pragma unroll
@@ -952,6 +968,7 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 ++nu;
             }
             constexpr int kOut = HD / kRowGroups;
+            const float undo = p.scale * one_over(f);
             const int col = grp * kOut;
             __nv_bfloat16* const dst = dq + u.s.b * p.dq.b + (int64_t)(u.s.q0 + i) * p.dq.n + u.h * p.dq.h + col;
             float* const part = P.part0 + (int64_t)u.split * p.B * p.H * p.Nq * HD + at * HD + col;
@@ -961,16 +978,15 @@ causal_dq_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant__
                 if (u.n > 0) {
                     tmem_ld16(tm_dq + lanes + col + c0, x);
                     tmem_wait_ld();
-                }
-                if (u.n == 0 || !sees) {           // (zero, whatever the row's masked zeros met in K)
+                } else {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[e] = 0u;
                 }
                 if (!mine) continue;
-                if constexpr (F16) {
-                    const float undo = p.scale / f;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * undo);
+                for (int e = 0; e < 16; ++e) {
+                    if constexpr (F16) x[e] = __float_as_uint(__uint_as_float(x[e]) * undo);
+                    x[e] = sees + row < 0 ? 0u : x[e];           // (zero, whatever the row's masked zeros met in K)
                 }
                 if (P.splits > 1) {
 #pragma unroll
@@ -1066,7 +1082,7 @@ inline BwdPlan plan_bwd(const CParams& c, bool f16) {
     f.part_v = take(f.splits_k > 1 ? (size_t)f.splits_k * c.B * c.Hkv * c.Nk * tile_columns(c.D) * 4 : 0);
     // (blocks that fill the multiprocessors, with a few rows a thread)
     const int64_t blocks = ((int64_t)c.B * c.H * c.Nq + (int64_t)c.B * c.Hkv * c.Nk) / (128LL * c.S) + 1;
-    f.parts = (int)(blocks < 256 ? blocks : 256);
+    f.parts = (int)(blocks < kMostParts ? blocks : kMostParts);
     if (f.parts > ceil_div(8 * sms, c.S)) f.parts = ceil_div(8 * sms, c.S);
     f.norms = take(f16 ? (size_t)c.S * f.parts * sizeof(float2) : 0);
     f.bytes = at;

@@ -347,8 +347,9 @@ causal_few_kernel(const __grid_constant__ FewParams P, const __nv_bfloat16* __re
             }
             return t;
         };
-        // O and LSE of row rho, columns d .. d + 3, of which t is the sum; `none`: the row has seen no key
+        // O and LSE of row rho, columns d .. d + 3, of which t is the sum; `none`: the row has seen no key (or all scores are -inf)
         auto store = [&](int rho, int d, float4 t, float top, float sum, bool none) {
+            none = none || sum == 0.f;
             const int i = rho / p.G, h = hk * p.G + rho - i * p.G;
             const int64_t at = ((int64_t)s.b * p.H + h) * p.Nq + s.q0 + i;
             const float ll = none ? -INFINITY : (top + log2f(sum)) * kLn2, inv = none ? 0.f : 1.f / sum;

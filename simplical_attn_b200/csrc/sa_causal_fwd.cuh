@@ -508,7 +508,7 @@ causal_fwd_tc_kernel(const __grid_constant__ FwdParams P, const __grid_constant_
             const bool mine = r < P.row_tiles && i < u.s.nq;
             const int64_t at = ((int64_t)u.s.b * p.H + u.h) * p.Nq + u.s.q0 + i;
             const int64_t rows = (int64_t)p.B * p.H * p.Nq;
-            const bool none = see < 0 || mt == 0;                    // no key (of this share)
+            const bool none = see < 0 || mt == 0 || l == 0.f;        // no key (of this share), or all scores are -inf
             if (mt > 0) {
                 mbar_wait<kOReady>(rb, nu & 1, wctx, 15);
                 tc_fence_after();

@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(kGenThreads) causal_fwd_kernel(const CParams p
             const int i = i0 + 4 * ty + r;
             const float sum = half_sum(l[r]);
             if (i < s.nq) {
-                const bool none = min(i + s.off(), j_end - 1) < j_begin;
+                const bool none = min(i + s.off(), j_end - 1) < j_begin || sum == 0.f;        // (or all scores are -inf)
                 const float ll = none ? -INFINITY : m[r] + logf(sum);
                 if (shares > 1) {
                     if (!none) store_row<float, DP>(part_o + (at.share * rows + row0 + i) * DP, acc[r], 1.f / sum, tx, p.D);
@@ -279,6 +279,9 @@ __global__ void __launch_bounds__(256) causal_delta_kernel(const CParams p, cons
     sum = warp_sum(sum);
     if (lane == 0) delta[((int64_t)b * p.H + h) * p.Nq + i] = sum;
 }
+
+// The LSE that a row's scores are taken from: with that of a row whose scores are all -inf every P is zero, as in the forward.
+__device__ __forceinline__ float lse_of_weights(float lse) { return lse == -INFINITY ? INFINITY : lse; }
 
 // P and dS of a tile of queries i0.. and keys j0..: zero outside the mask.  (exp of a score against the row's LSE: a row that
 // sees no key has no score inside the mask.)
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(kGenThreads) causal_dq_kernel(const CParams p,
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int i = i0 + 4 * ty + r;
-            ls[r] = i < s.nq ? lse[i] : 0.f;
+            ls[r] = i < s.nq ? lse_of_weights(lse[i]) : 0.f;
             dl[r] = i < s.nq ? delta[i] : 0.f;
 #pragma unroll
             for (int e = 0; e < L::kDpt; ++e) acc[r][e] = 0.f;
@@ -408,7 +411,7 @@ __global__ void __launch_bounds__(kGenThreads) causal_dkv_kernel(const CParams p
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = i0 + 4 * ty + r;
-                ls[r] = i < s.nq ? lse[row + i] : 0.f;
+                ls[r] = i < s.nq ? lse_of_weights(lse[row + i]) : 0.f;
                 dl[r] = i < s.nq ? delta[row + i] : 0.f;
             }
             __syncthreads();

@@ -11,10 +11,10 @@ constexpr int kTile = 128;            // rows of a query tile = lanes of tensor 
 
 // 2^x of two values on the FMA pipes, for x up to 100: x = n + f with n whole and |f| <= 1/2, 2^f by a polynomial of degree 4
 // (minimax of the relative error, 2.7e-6, fitted by reweighted least squares at Chebyshev points), 2^n from the bits of n.  Below
-// -126 it is 2^-126 or less than that times two; NaN stays NaN.
+// -126.5 it is zero (n = -127 leaves no bit); NaN stays NaN.
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
     const float kRound = 12582912.f;                 // 1.5 * 2^23: adding it leaves n in the low bits
     const float2 r = __fadd2_rn(x, make_float2(kRound, kRound)), n = __fadd2_rn(r, make_float2(-kRound, -kRound));
     const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import simplical_attn_b200 as sab
-from tests.test_causal import algo, make  # noqa: F401 (algo: fixture)
+from tests.test_causal import algo, make, step  # noqa: F401 (algo: fixture)
 
 gpu = pytest.mark.gpu
 
@@ -41,3 +41,31 @@ def test_a_row_that_is_not_finite_stays_so(D, dtype, algo):  # noqa: F811
     v[280, :, 5] = math.inf
     got = sab.causal_attention(q, k, v, cu_q=cu_q, cu_k=cu_k)
     assert torch.isnan(got[290]).all() and (got[280:290, :, 5] == math.inf).all() and (got[291:, :, 5] == math.inf).all()
+
+
+# B, N, M: whole walks of many units, shares joined by a kernel, a few rows in one share, in a cluster, in many shares
+@gpu
+@pytest.mark.parametrize("shape", [(5, 300, 300), (1, 130, 3000), (1, 2, 40), (1, 2, 700), (1, 2, 20000)])
+@pytest.mark.parametrize("D,dtype", [(64, "bf16"), (128, "bf16"), (64, "fp32")])
+def test_scores_of_minus_infinity(shape, D, dtype, algo):  # noqa: F811
+    """A query all of whose scores overflow to -inf weighs no key, as if it saw none: O = 0, LSE = -inf and no gradient, however the
+    keys are cut up.  Beside finite scores such a key has weight zero."""
+    B, N, M = shape
+    H, Hkv = (32, 32) if B > 1 else (4, 2)
+    (q, k, v, d_o), _, _ = make([(N, M)] * B, H, Hkv, D, dtype, seed=54)
+    q, k, v, d_o = (t.view(B, -1, *t.shape[1:]) for t in (q, k, v, d_o))
+    row = N // 2
+    q, k = q.clone(), k.clone()
+    k[..., 0], q[..., 0] = -1e20, 0          # (products of zero with the big elements change nothing: the other rows keep their scores)
+    base = step(q, k, v, d_o)
+    q[:, row, :, 0] = 1e25
+    got = step(q, k, v, d_o)
+    assert not got["o"][:, row].any() and (got["lse"][:, :, row] == -math.inf).all() and not got["dq"][:, row].any()
+    rest = [i for i in range(N) if i != row]
+    assert torch.equal(got["o"][:, rest], base["o"][:, rest]) and torch.equal(got["dq"][:, rest], base["dq"][:, rest])
+    # the row takes part in no gradient: those of K and V are what they are without its dO
+    d_o = d_o.clone()
+    d_o[:, row] = 0
+    q[:, row] = 0
+    without = step(q, k, v, d_o)
+    assert torch.equal(got["dv"], without["dv"]) and torch.equal(got["dk"], without["dk"])
