@@ -62,20 +62,16 @@ struct BwdParams {
 // of this.)  With M the largest |dO_i . V_j| of a sequence, |dS_ij| = P_ij |sum_k P_ik (dP_ij - dP_ik)| <= 2 M P_ij (1 - P_ij) <= M / 2,
 // and M is at most the product of the longest rows of dO and V.  For rows of normal values the factor makes dS about 2^13 P.
 constexpr float kPFactor = 32768.f, kPFactorLog2 = 15.f;
-constexpr int kMostParts = 256;
+constexpr int kMostParts = 128;
 // The factor of a sequence (a whole warp): from the squares of the two lengths a power of two f with sqrt(do2 v2) / 2 f in [2^14, 2^15).
 __device__ __forceinline__ float ds_factor(const BwdParams& P, int sequence) {
     float do2 = 0.f, v2 = 0.f;
-    float2 t[kMostParts / 32];
 #pragma unroll
-    for (int x = 0; x < kMostParts / 32; ++x) {        // (all loads under way together: this stands at the start of a unit)
-        const int y = 32 * x + (threadIdx.x & 31);
-        t[x] = y < P.parts ? P.norms[(int64_t)sequence * P.parts + y] : make_float2(0.f, 0.f);
-    }
-#pragma unroll
-    for (int x = 0; x < kMostParts / 32; ++x) {
-        do2 = fmaxf(do2, t[x].x);
-        v2 = fmaxf(v2, t[x].y);
+    for (int x = 0; x < kMostParts; x += 32) {         // (loads under way together: this stands at the start of a unit)
+        const int y = x + (threadIdx.x & 31);
+        const float2 t = y < P.parts ? P.norms[(int64_t)sequence * P.parts + y] : make_float2(0.f, 0.f);
+        do2 = fmaxf(do2, t.x);
+        v2 = fmaxf(v2, t.y);
     }
     // (not negative: ordered as their bits are)
     do2 = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(do2)));
