@@ -190,7 +190,8 @@ def causal_attention(q, k, v, scale: Optional[float] = None, *, cu_q: Optional[t
     What lies in keys that a query does not see, in rows outside the sequences and in other sequences does not reach a result,
     NaN and infinities included.  The gradients keep to that between sequences; within one, an element that is not finite may reach
     gradients across the mask, at most 254 rows away.  They are written without atomics: equal calls give equal bits.  There is no
-    second derivative.  A backward pass is captured into a graph under torch's own condition, that no eager graph of the same leaves is
+    second derivative.  For 16-bit tensors a call with a history keeps, beside Q, K, V, O and the LSE, what rounding took from O: one more
+    tensor of O's size until its backward pass.  A backward pass is captured into a graph under torch's own condition, that no eager graph of the same leaves is
     alive.
     """
     if scale is None:

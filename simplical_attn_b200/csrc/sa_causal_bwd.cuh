@@ -9,7 +9,7 @@
 // written that is not a result, and equal calls give equal bits.
 //
 // Both are persistent, with groups of four warps (compute) each at a share of a tile's columns and a row of tensor memory per
-// thread -- two groups (dK, dV) or four (dQ: 700 -> 580 us at D = 64 of the size below; for dK, dV no difference) --, then a warp
+// thread -- two groups (dK, dV) or four (dQ: 17 % faster at D = 64; for dK, dV no difference) --, then a warp
 // issuing MMAs, one TMA loads, one guarding: it zeroes the rows behind a sequence's end in tiles that
 // the MMAs sum over (they belong to the next sequence, and a masked zero times its NaN would not be zero) and the queries that see
 // no key, and in the dK / dV kernel loads LSE and Delta of the query tile.  P and dS go from registers to tensor memory and from there into the MMA as
@@ -19,8 +19,9 @@
 // computed.  MMA cycles per pair of tiles at D = 128: 2048 (dK, dV), 1536 (dQ); exponentials take 1024 of either, and operand reads
 // and TMA writes of shared memory 2290 and 1792.
 //
-// Measured, bf16 B 2 N 8192 H 16/4: D 128 dK, dV 821 us (1340 TFLOP/s of its four products), dQ 644 us (1280 of three); D 64 745 and
-// 565 us.  Steps take about 2890 and 2310 cycles at D 128.
+// Measured back to back for a second, bf16 B 2 N 8192 H 16/4: D 128 dK, dV 961 us (1144 TFLOP/s of its four products, under the power
+// cap; 840 with pauses), dQ 730 us (1130 of three; 670), Delta 42; D 64 660, 492 and 22 us.  In fp16 5 % more at D 128.  Under a
+// profiler a step takes about 3220 and 2520 cycles at D 128 (1.64 GHz, tensor pipe 67 and 65 % active), 2590 and 1910 at D 64.
 #pragma once
 
 #include "sa_causal_fwd.cuh"
@@ -61,6 +62,8 @@ struct BwdParams {
 // sequence, as large as overflow allows; both are undone in fp32 where rows are written.  (bf16 has the exponents of fp32: nothing
 // of this.)  With M the largest |dO_i . V_j| of a sequence, |dS_ij| = P_ij |sum_k P_ik (dP_ij - dP_ik)| <= 2 M P_ij (1 - P_ij) <= M / 2,
 // and M is at most the product of the longest rows of dO and V.  For rows of normal values the factor makes dS about 2^13 P.
+// Costs: the longest rows are found by blocks beside Delta's, 2 us at B 2 N 512 H 4 and 8 of 219 for packed sequences of 1999 to 378
+// rows (H 16/4 D 64), and 3 % at B 2 N 8192 H 16/4 D 128.
 constexpr float kPFactor = 32768.f, kPFactorLog2 = 15.f;
 constexpr int kMostParts = 128;
 // The factor of a sequence (a whole warp): from the squares of the two lengths a power of two f with sqrt(do2 v2) / 2 f in [2^14, 2^15).
@@ -1061,7 +1064,7 @@ inline BwdPlan plan_bwd(const CParams& c, bool f16) {
     f.items_q = packed ? list_capacity(c.Nq, kTile, c.S) : (int64_t)ceil_div(c.Nq, kTile) * c.S;
     f.items_k = packed ? list_capacity(c.Nk, kTile, c.S) : (int64_t)ceil_div(c.Nk, kTile) * c.S;
     const int sms = host::sm_count();
-    // (a step of either kernel takes about 1.3 us, adding shares 5 for a tensor and the partial rows' way through memory)
+    // (a step of either kernel takes about 1.3 us at D 128, which is taken for every head dim; adding shares 5 for a tensor and the partial rows' way through memory)
     const double row_us = (double)c.B * tile_columns(c.D) * 8 / 5e6;
     const int steps_q = ceil_div(c.max_k, kTile);
     f.splits_q = plan_shares((double)f.items_q * c.H, steps_q, mean_steps(c, steps_q), sms, 16, 3.8, row_us * c.H * c.Nq / 1.3);

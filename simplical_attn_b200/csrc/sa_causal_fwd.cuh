@@ -15,10 +15,12 @@
 // at D = 128 it waits for P V.
 //
 // Per pair of query tiles and 128 keys at D = 128 the MMAs take 2048 cycles (128 x 128 x 16 in 64) and so do the exponentials
-// (16 per clock).  Measured, bf16 B 2 N 8192 H 16/4: 418 us at D 128 (1316 TFLOP/s; about 3000 cycles a pair, tensor pipe 60 %
-// active, 1.58 GHz under load: what is left is the chain from S through the softmax to P V of each query tile), 373 us at D 64
-// (737; the exponentials take 66 % of what they could).  With two threads to a row (sixteen softmax warps) 452 and 371 us; with
-// exponentials on the FMA pipes as well, every eighth to every third pair, 3 to 10 % slower.
+// (16 per clock).  Measured back to back for a second, bf16 B 2 N 8192 H 16/4: 493 us at D 128 (1116 TFLOP/s under the power cap;
+// 470 with pauses; 525 where the low part of O is wanted, too), 375 us at D 64 (732 TFLOP/s).  Under a profiler at 1.60 GHz a pair
+// takes about 3400 cycles at D 128, the tensor pipe is 63 % active: what is left is the chain from S through the softmax to P V of
+// each query tile.  At D 64 the exponentials take 70 % of what they could.  Dropped, each against the kernel of its time: two threads
+// to a row (sixteen softmax warps: 8 % slower at D 128, no difference at D 64), exponentials on the FMA pipes as well, every eighth
+// to every third pair (3 to 10 % slower).
 //
 // Masked scores become -inf whatever they are, so P is an exact zero there; V rows of tiles with masked scores might still meet
 // that zero as NaN or infinity.  The guard warp looks through those tiles before their MMAs: rows behind the sequence's
@@ -688,7 +690,8 @@ inline FwdPlan plan_fwd(const CParams& c) {
     auto items = [&](int tiles) {
         return c.cu_q != nullptr ? list_capacity(c.Nq, kTile * tiles, c.S) : (int64_t)ceil_div(c.Nq, kTile * tiles) * c.S;
     };
-    // A key tile takes a pair of query tiles 1.95 us and a single one 1.75 (D 128; nothing overlaps its softmax); joining shares
+    // A key tile takes a pair of query tiles 1.95 us and a single one 1.75 (measured at D 128 and taken for every head dim, though at
+    // D 64 a pair takes 1.6; nothing overlaps a single one's softmax); joining shares
     // takes 8 us and the partial rows' way through memory.
     const int tiles = ceil_div(c.max_k, kTile);
     const double mean = mean_steps(c, tiles), each = (double)c.B * c.H * c.Nq * tile_columns(c.D) * 8 / 5e6;

@@ -164,7 +164,8 @@ def rotary_positions(tensors: Union[torch.Tensor, Sequence[torch.Tensor]], frequ
     `magnitude` scales the rotated part; `inverse` turns back.  Returns a tensor for a tensor, else a tuple.
 
     `out` (a tensor, or as many as `tensors`) takes the results; an output may be its input itself, which then is turned in
-    place, and must not overlap it otherwise.  Such a call records no gradient and refuses tensors that require one.
+    place, and must not overlap it otherwise.  Such a call records no gradient and refuses tensors that require one; it needs the
+    native binding and plain tensors (no trace, no functorch transform, no subclass).
     """
     one = isinstance(tensors, torch.Tensor)
     xs = (tensors,) if one else tuple(tensors)
