@@ -58,15 +58,16 @@ struct BwdParams {
 
 // fp16 keeps all of its bits from 2^-14 to 2^16 only.  Over n keys P is about 1 / n and dS that times the size of dO and V, so as they
 // are both would lose bits or vanish although the gradients do not (dQ off by 3 % at 4096 keys and |dO| = 10^-3, by 29 % at
-// 10^-4).  P therefore goes into dV times 2^15, and dS into dQ and dK without the softmax scale and times a power of two of its
-// sequence, as large as overflow allows; both are undone in fp32 where rows are written.  (bf16 has the exponents of fp32: nothing
+// 10^-4).  P therefore goes into dV times 2^12, and dS into dQ and dK without the softmax scale and times a power of two of its
+// sequence that brings it to at most 2^12; both are undone in fp32 where rows are written.  (bf16 has the exponents of fp32: nothing
 // of this.)  With M the largest |dO_i . V_j| of a sequence, |dS_ij| = P_ij |sum_k P_ik (dP_ij - dP_ik)| <= 2 M P_ij (1 - P_ij) <= M / 2,
-// and M is at most the product of the longest rows of dO and V.  For rows of normal values the factor makes dS about 2^13 P.
+// and M is at most the product of the longest rows of dO and V.  For rows of normal values the factor makes dS about 2^10 P.
+// 2^12 leaves a factor of 16: scores of 10^7 and more are off by several units in 32 bits, here and in the LSE, and P may be above 1.
 // Costs: the longest rows are found by blocks beside Delta's, 2 us at B 2 N 512 H 4 and 8 of 219 for packed sequences of 1999 to 378
 // rows (H 16/4 D 64), and 3 % at B 2 N 8192 H 16/4 D 128.
-constexpr float kPFactor = 32768.f, kPFactorLog2 = 15.f;
+constexpr float kPFactor = 4096.f, kPFactorLog2 = 12.f;
 constexpr int kMostParts = 128;
-// The factor of a sequence (a whole warp): from the squares of the two lengths a power of two f with sqrt(do2 v2) / 2 f in [2^14, 2^15).
+// The factor of a sequence (a whole warp): from the squares of the two lengths a power of two f with sqrt(do2 v2) / 2 f in [2^11, 2^12).
 __device__ __forceinline__ float ds_factor(const BwdParams& P, int sequence) {
     float do2 = 0.f, v2 = 0.f;
 #pragma unroll
@@ -82,7 +83,7 @@ __device__ __forceinline__ float ds_factor(const BwdParams& P, int sequence) {
     const float x = do2 * v2;                          // (2^-96 to 2^79)
     if (!(x > 0.f)) return 1.f;
     const int e = (__float_as_int(x) >> 23) - 127;     // x < 2^(e + 1)
-    return __int_as_float((16 - ((e + 2) >> 1) + 127) << 23);
+    return __int_as_float((13 - ((e + 2) >> 1) + 127) << 23);
 }
 
 __device__ __forceinline__ float one_over(float power_of_two) { return __int_as_float((254 << 23) - __float_as_int(power_of_two)); }
@@ -471,7 +472,7 @@ causal_dkv_tc_kernel(const __grid_constant__ BwdParams P, const __grid_constant_
         for (Walk w(P, p.Hkv); w.valid(); w.next()) {
             const ColUnit u = col_unit(P, w);
             ColStep st(u);
-            const float f = F16 ? ds_factor(P, u.s.id) / kPFactor : p.scale;        // of dP; P has 2^15 already (through its LSE)
+            const float f = F16 ? ds_factor(P, u.s.id) / kPFactor : p.scale;        // of dP; P has its factor already (through its LSE)
             const float2 sc = make_float2(f, f);
 #pragma unroll 1
             for (int it = 0; it < u.n; ++it, ++n, st.next(u)) {

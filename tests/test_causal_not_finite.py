@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import simplical_attn_b200 as sab
+from tests import causal_ref
 from tests.test_causal import algo, make, step  # noqa: F401 (algo: fixture)
 
 gpu = pytest.mark.gpu
@@ -69,3 +70,20 @@ def test_scores_of_minus_infinity(shape, D, dtype, algo):  # noqa: F811
     q[:, row] = 0
     without = step(q, k, v, d_o)
     assert torch.equal(got["dv"], without["dv"]) and torch.equal(got["dk"], without["dk"])
+
+
+@gpu
+@pytest.mark.parametrize("N,M", [(300, 300), (130, 3000), (2, 700)])
+def test_scores_of_minus_infinity_beside_others(N, M, algo):  # noqa: F811
+    """The keys whose scores are -inf have weight zero, whole tiles of them before the first other one included."""
+    (q, k, v, d_o), (cu_q, cu_k), _ = make([(N, M)], 2, 1, 64, "bf16", seed=55)
+    row, first = N - 1, M - M // 4
+    k[:, :, 0], q[:, :, 0] = 0, 0
+    k[:first, :, 0] = -1e20
+    q[row, :, 0] = 1e25
+    got = step(q, k, v, d_o, cu_q=cu_q, cu_k=cu_k)
+    val, err = causal_ref.reference(q[row:row + 1] * (torch.arange(64, device="cuda") > 0), k[first:] * (torch.arange(64, device="cuda") > 0), v[first:], None,
+                                    [(0, 1, 0, M - first)], 0.125)
+    causal_ref.check(got["o"][row:row + 1], val["o"], err["o"], "o")
+    causal_ref.check(got["lse"][:, row:row + 1], val["lse"], err["lse"], "lse")
+    assert torch.isfinite(got["dq"][:row]).all() and torch.isfinite(got["dv"]).all()

@@ -70,3 +70,14 @@ def test_fp16_gradients_do_not_depend_on_other_sequences(packed, algo):  # noqa:
     two = step(q, k, v, d_o, **kw)
     for n in one:
         assert torch.equal(one[n], middle(two[n])), n
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_gradients_at_huge_scores(D, algo):  # noqa: F811
+    """Scores of some 10^6, which 32 bits hold to a unit or so: P may come out above 1, and nothing overflows for it."""
+    (q, k, v, d_o), (cu_q, cu_k), _ = make([(300, 300)], 2, 1, D, "fp16", seed=44, spread=1.0)
+    q, k = q * 700, k * 700
+    got = step(q, k, v, d_o, cu_q=cu_q, cu_k=cu_k)
+    assert float((q.float()[:, 0] @ k.float()[:, 0].T).abs().max()) * D ** -0.5 > 1e6
+    assert all(torch.isfinite(t).all() for t in got.values())
